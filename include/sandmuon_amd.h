@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define SMX_ABI_VERSION 5
+#define SMX_ABI_VERSION 6
 
 enum smx_status {
   SMX_OK = 0,
@@ -499,6 +499,174 @@ int smx_mfma_peak(int32_t dtype, int32_t blocks, int64_t iters,
  * [0, 2] (then nothing changes).
  * ------------------------------------------------------------------ */
 int smx_s8_tile_geometry(int32_t policy);
+
+/* ------------------------------------------------------------------ *
+ * Activations kept in 8 bits for the backward pass (no counterpart in the
+ * reference, whose statistics and update they leave as they are).  The
+ * elements of a row in blocks of 32 neighbours share a scale byte b; a
+ * code stands for code * 2^(b - 127).  With E the exponent of a block's
+ * largest magnitude:
+ *   SMX_ACT8_INT8: b = max(E + 121, 1), code = round(x / scale) to nearest
+ *     even in [-127, 127]: an error of half a step, 2^-7 of the block's
+ *     largest magnitude or less (a whole step where that rounds to 128);
+ *   SMX_ACT8_E4M3: b = max(E + 120, 10) (E = 127: 248, codes to 120), code = x / scale
+ *     rounded to a float of 4 exponent and 3 fraction bits: 2^-4 of every
+ *     element down to 2^-13 of the largest, for blocks with outliers.
+ * A code's value is exact in BF16 and FP32.  A block with an infinity or a
+ * NaN gets b = 255 and reads back as NaN.
+ *
+ * codes are [rows, pitch] bytes, 16-byte aligned, and scales [rows, pitch /
+ * 32], with pitch = cols rounded up to a multiple of 32 (the padding's codes
+ * are zero).  Tensors are [rows, cols] views with unit column stride.
+ * ------------------------------------------------------------------ */
+enum smx_act8_format { SMX_ACT8_INT8 = 0, SMX_ACT8_E4M3 = 1 };
+
+int smx_act8_encode(const void *x, int dtype, int64_t rows, int64_t cols,
+                    int64_t row_stride, int fmt, uint8_t *codes,
+                    uint8_t *scales, int64_t pitch, void *stream);
+int smx_act8_decode(const uint8_t *codes, const uint8_t *scales, int fmt,
+                    int64_t rows, int64_t cols, int64_t pitch, void *out,
+                    int dtype, int64_t out_stride, void *stream);
+
+/* smx_act8_gelu: y = GELU(h), exact form, in h's type, with h kept in 8 bits
+ * for smx_act8_gelu_backward and, unless y_codes and y_scales are null, y
+ * kept as it is stored (rounded to its type) for smx_act8_wgrad of the Linear
+ * that receives it.  smx_act8_gelu_backward: dh = dy * GELU'(kept h). */
+int smx_act8_gelu(const void *h, int dtype, int64_t rows, int64_t cols,
+                  int64_t row_stride, int fmt, void *y, int64_t y_stride,
+                  uint8_t *h_codes, uint8_t *h_scales, uint8_t *y_codes,
+                  uint8_t *y_scales, int64_t pitch, void *stream);
+int smx_act8_gelu_backward(const void *dy, int dtype, int64_t rows,
+                           int64_t cols, int64_t dy_stride,
+                           const uint8_t *h_codes, const uint8_t *h_scales,
+                           int fmt, int64_t pitch, void *dh,
+                           int64_t dh_stride, void *stream);
+
+/* smx_act8_wgrad: the weight and bias gradients of a Linear whose input is
+ * kept, dw[n, k] = sum over rows of delta[row, n] * kept[row, k] and
+ * db[n] = sum over rows of delta[row, n] (db may be null), both contiguous of
+ * `out_dtype`, rounded once from FP32 sums.  Products are exact: a BF16
+ * delta times a code's value; an FP16 or FP32 delta as the sum of its two or
+ * three BF16 parts.  rows = 0 gives zeros.  `workspace`: 256-byte aligned,
+ * smx_act8_wgrad_workspace_bytes(rows, n, k, dtype) bytes (none needed: 0). */
+int64_t smx_act8_wgrad_workspace_bytes(int64_t rows, int64_t n, int64_t k,
+                                       int dtype);
+int smx_act8_wgrad(const void *delta, int dtype, int64_t rows, int64_t n,
+                   int64_t delta_stride, const uint8_t *codes,
+                   const uint8_t *scales, int fmt, int64_t k, int64_t pitch,
+                   void *dw, void *db, int out_dtype, void *workspace,
+                   int64_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------ *
+ * RMS norm of every query and key head with its rotary position rotation
+ * (no counterpart in the reference):
+ *   n = x * rsqrt(mean(x^2) + eps) * weight;
+ *   the first `rot` elements of n in pairs (a, b), turned by the position's
+ *   angle: (a cos - b sin, a sin + b cos).
+ * SMX_ROTARY_HALF pairs element p with p + rot/2, SMX_ROTARY_INTERLEAVED 2p
+ * with 2p + 1.  cos and sin are [table_rows, rot/2] FP32.  A token's position
+ * is positions[b * pos_stride[0] + t * pos_stride[1]], or position0 + t where
+ * positions is null; one outside the tables gives NaN in the turned elements.
+ * x, y, dy are [batch, seq, heads, dim] with the given strides (elements) of
+ * batch, seq and head, and a unit last one; y may be x.  A side with heads =
+ * 0 is left out.  Backward: x and weight as in the forward, dy the cotangent
+ * of its result; y receives dx, dw (unless null) the weight's gradient, in
+ * the weight's type.
+ * ------------------------------------------------------------------ */
+enum smx_rotary_style { SMX_ROTARY_HALF = 0, SMX_ROTARY_INTERLEAVED = 1 };
+
+typedef struct smx_qk_side {
+  const void *x;
+  const void *weight; /* [dim] of weight_dtype, or NULL: ones */
+  const void *dy;
+  void *y;
+  void *dw;
+  int64_t heads;
+  int64_t x_stride[3], y_stride[3], dy_stride[3];
+  int32_t weight_dtype, pad_;
+} smx_qk_side;
+
+typedef struct smx_qk_desc {
+  smx_qk_side q, k;
+  const float *cos, *sin;
+  const int64_t *positions;
+  int64_t pos_stride[2];
+  int64_t position0, table_rows;
+  int64_t batch, seq, dim, rot;
+  double eps;
+  int32_t dtype, style;
+} smx_qk_desc;
+
+int smx_qk_norm_rotary(const smx_qk_desc *desc, void *stream);
+/* The backward's workspace (16-byte aligned), needed where a dw is given. */
+int64_t smx_qk_workspace_bytes(int64_t dim);
+int smx_qk_norm_rotary_backward(const smx_qk_desc *desc, void *workspace,
+                                int64_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------ *
+ * Losses on logits [batch, seq, vocab] (unit last stride, batch_stride and
+ * row_stride elements; no counterpart in the reference).  targets [batch,
+ * seq], mask [batch, seq] of bytes (null: every token is live) and the
+ * per-token floats are contiguous.  A token whose mask is 0 is not looked at:
+ * its log probability is 0, its gradient 0.  A live token's target outside
+ * the vocabulary makes its log probability and gradient NaN.  Gradients to
+ * the logits are contiguous, of the logits' type.
+ *
+ * smx_token_logprobs: logprobs = z[target] - lse(z); stats (or null) receives
+ * each row's maximum and sum of exp(z - maximum), [batch, seq, 2], for the
+ * backward (8-byte aligned).  smx_token_logprobs_backward: dlogits = coef * (onehot(target)
+ * - softmax(z)), coef read at b * coef_batch_stride + t * coef_row_stride and
+ * multiplied by *scale (device, or null).
+ * ------------------------------------------------------------------ */
+int smx_token_logprobs(const void *logits, int dtype, int64_t batch,
+                       int64_t seq, int64_t vocab, int64_t batch_stride,
+                       int64_t row_stride, const int64_t *targets,
+                       const uint8_t *mask, float *logprobs, float *stats,
+                       void *stream);
+int smx_token_logprobs_backward(const void *logits, int dtype, int64_t batch,
+                                int64_t seq, int64_t vocab,
+                                int64_t batch_stride, int64_t row_stride,
+                                const int64_t *targets, const uint8_t *mask,
+                                const float *stats, const float *coef,
+                                int64_t coef_batch_stride,
+                                int64_t coef_row_stride, const float *scale,
+                                void *dlogits, void *stream);
+
+/* smx_policy_loss: the clipped policy loss with a KL term, and its gradient
+ * to the logits, in one pass.  With r = exp(lp - old) (1 where old_logprobs is
+ * null), A the advantage and g = ref - lp, a live token's term is
+ *   -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^g - g - 1)
+ * (the last part left out where ref_logprobs is null), and the loss is
+ * `scale` times the mean of the terms over the live tokens
+ * (SMX_MEAN_TOKEN), or over the sequences with live tokens of their means
+ * (SMX_MEAN_SEQUENCE); 0 where no token is live.  dlogits may be null. */
+enum smx_loss_reduction { SMX_MEAN_TOKEN = 0, SMX_MEAN_SEQUENCE = 1 };
+int64_t smx_policy_loss_workspace_bytes(int64_t batch, int64_t seq);
+int smx_policy_loss(const void *logits, int dtype, int64_t batch, int64_t seq,
+                    int64_t vocab, int64_t batch_stride, int64_t row_stride,
+                    const int64_t *targets, const uint8_t *mask,
+                    const float *old_logprobs, const float *ref_logprobs,
+                    const float *advantages, int64_t adv_batch_stride,
+                    int64_t adv_row_stride, double clip_low, double clip_high,
+                    double kl_coef, int reduction, double scale, float *loss,
+                    float *logprobs, void *dlogits, void *workspace,
+                    int64_t workspace_bytes, void *stream);
+
+/* smx_preference_loss: from token log probabilities [2 * pairs, seq], the
+ * chosen sequences first: with m = beta * (gain of the chosen - gain of the
+ * rejected), gain the sum of a sequence's live logprobs - ref_logprobs,
+ *   loss = mean of -(1 - s) log sigmoid(m) - s log sigmoid(-m),
+ * s = label_smoothing; margins receives m, coef [2 * pairs] the derivative of
+ * the loss by a live token's log probability (smx_token_logprobs_backward's
+ * coef with strides 1 and 0). */
+int smx_preference_loss(const float *logprobs, const float *ref_logprobs,
+                        const uint8_t *mask, int64_t pairs, int64_t seq,
+                        double beta, double label_smoothing, float *loss,
+                        float *margins, float *coef, void *stream);
+
+/* x *= *scale on n contiguous values (scale on the device; 1 leaves x as it
+ * is and reads nothing else). */
+int smx_scale(void *x, int dtype, int64_t n, const float *scale, void *stream);
 
 #ifdef __cplusplus
 }

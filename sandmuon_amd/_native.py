@@ -18,7 +18,7 @@ from typing import List, Optional, Sequence
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libsandmuon_amd.so"
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 SMX_F32, SMX_BF16, SMX_F16, SMX_F64 = 0, 1, 2, 3
 S8_FP32, S8_COMP_BF16, S8_MIXED = 0, 1, 2
@@ -61,6 +61,19 @@ class MatrixDesc(ctypes.Structure):
                 ("inv_row", c_void_p), ("inv_col", c_void_p), ("z", c_void_p), ("kappa", c_void_p),
                 ("rows", c_int64), ("cols", c_int64), ("lr", c_double), ("momentum_beta", c_double),
                 ("grad_dtype", c_int32), ("param_dtype", c_int32)]
+
+
+class QkSide(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("weight", c_void_p), ("dy", c_void_p), ("y", c_void_p), ("dw", c_void_p),
+                ("heads", c_int64), ("x_stride", c_int64 * 3), ("y_stride", c_int64 * 3), ("dy_stride", c_int64 * 3),
+                ("weight_dtype", c_int32), ("pad_", c_int32)]
+
+
+class QkDesc(ctypes.Structure):
+    _fields_ = [("q", QkSide), ("k", QkSide), ("cos", c_void_p), ("sin", c_void_p), ("positions", c_void_p),
+                ("pos_stride", c_int64 * 2), ("position0", c_int64), ("table_rows", c_int64), ("batch", c_int64),
+                ("seq", c_int64), ("dim", c_int64), ("rot", c_int64), ("eps", c_double), ("dtype", c_int32),
+                ("style", c_int32)]
 
 
 # The descriptors' bytes, field by field in order (native alignment; the
@@ -134,6 +147,33 @@ SIGNATURES = {
     "smx_s8_timing_read": (c_int32, [ctypes.POINTER(ctypes.c_float), ctypes.POINTER(c_int32),
                                      ctypes.POINTER(c_double), c_int32]),
 }
+
+_LOGITS = [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p]
+SIGNATURES.update({
+    "smx_act8_encode": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int64,
+                                c_void_p]),
+    "smx_act8_decode": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64,
+                                c_void_p]),
+    "smx_act8_gelu": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p,
+                              c_void_p, c_void_p, c_int64, c_void_p]),
+    "smx_act8_gelu_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64,
+                                       c_void_p, c_int64, c_void_p]),
+    "smx_act8_wgrad_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
+    "smx_act8_wgrad": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int64,
+                               c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p]),
+    "smx_qk_norm_rotary": (c_int, [ctypes.POINTER(QkDesc), c_void_p]),
+    "smx_qk_workspace_bytes": (c_int64, [c_int64]),
+    "smx_qk_norm_rotary_backward": (c_int, [ctypes.POINTER(QkDesc), c_void_p, c_int64, c_void_p]),
+    "smx_token_logprobs": (c_int, [*_LOGITS, c_void_p, c_void_p, c_void_p]),
+    "smx_token_logprobs_backward": (c_int, [*_LOGITS, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                            c_void_p]),
+    "smx_policy_loss_workspace_bytes": (c_int64, [c_int64, c_int64]),
+    "smx_policy_loss": (c_int, [*_LOGITS, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_double, c_double, c_double,
+                                c_int, c_double, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "smx_preference_loss": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_double, c_double, c_void_p,
+                                    c_void_p, c_void_p, c_void_p]),
+    "smx_scale": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p]),
+})
 
 _lib: Optional[ctypes.CDLL] = None
 _lock = threading.Lock()

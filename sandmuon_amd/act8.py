@@ -1,0 +1,326 @@
+"""Activations kept in 8 bits for the backward pass.
+
+A Linear keeps its input, and a GELU its input, from the forward to the
+backward: for a GPT block that is most of the memory of a training step.
+Here they are kept in one byte an element and one scale byte per 32 (33/64 of
+bf16), and the backward passes read the bytes themselves:
+
+* ``encode`` / ``decode``: any [..., d] activation to 8 bits and back;
+* ``linear_backward``: a Linear's weight and bias gradients from the cotangent
+  and its kept input, on BF16 MFMAs (the kept values are exact in BF16);
+* ``gelu_forward`` / ``gelu_backward``: the exact GELU with its input (and, for
+  the Linear behind it, its output) kept in the same pass, and its gradient;
+* ``linear``, ``gelu``, ``mlp``: these as differentiable functions, under
+  autocast as torch's own; ``checkpoint_linears`` puts every selected
+  ``nn.Linear`` of a model on ``linear``.  The optimizer's statistics hooks see
+  the unrounded inputs and cotangents, as before.
+
+Formats.  The elements of a row in blocks of 32 neighbours share a power of
+two.  ``"int8"`` (the default) holds round(x / step) with a step of 2^-6 of the
+largest magnitude's power of two; ``"e4m3"`` holds a float of 3 fraction bits,
+for activations whose blocks hold outliers.  A block with an infinity or a NaN
+reads back as NaN.
+
+Only what the backward reads is rounded: outputs and input gradients of a
+Linear are those of torch, weight gradients those of the kept input, summed in
+FP32.  Double backward is not supported.
+"""
+from __future__ import annotations
+
+import types
+from typing import Callable, Optional, Tuple
+
+import torch
+import torch.nn.functional as F
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from . import _native
+from ._tensors import need_float, on_device, rows2d, same_device
+
+__all__ = ["Act8", "FORMATS", "checkpoint_linears", "decode", "encode", "gelu", "gelu_backward", "gelu_forward",
+           "linear", "linear_backward", "mlp"]
+
+FORMATS = {"int8": 0, "e4m3": 1}
+_BLOCK = 32
+
+
+def _fmt(fmt: str, what: str) -> int:
+    code = FORMATS.get(fmt)
+    if code is None:
+        raise ValueError(f"{what}: unknown 8-bit format {fmt!r}; expected one of {sorted(FORMATS)}")
+    return code
+
+
+class Act8:
+    """A kept activation: codes [rows, pitch] and scale bytes [rows, pitch /
+    32] in one buffer, with the activation's shape and format."""
+
+    __slots__ = ("data", "shape", "rows", "cols", "pitch", "fmt")
+
+    def __init__(self, shape, fmt: str, device):
+        self.shape = torch.Size(shape)
+        self.cols = self.shape[-1]
+        self.rows = self.shape[:-1].numel()
+        self.pitch = -(-self.cols // _BLOCK) * _BLOCK
+        self.fmt = fmt
+        self.data = torch.empty(self.rows * (self.pitch + self.pitch // _BLOCK), dtype=torch.uint8, device=device)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self.data[:self.rows * self.pitch].view(self.rows, self.pitch)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.data[self.rows * self.pitch:].view(self.rows, self.pitch // _BLOCK)
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel()
+
+    def _ptrs(self) -> Tuple[int, int]:
+        at = self.data.data_ptr()
+        return at, at + self.rows * self.pitch
+
+
+def _activation(x: torch.Tensor, what: str) -> torch.Tensor:
+    need_float(x, what)
+    if x.dim() < 1:
+        raise ValueError(f"{what}: expected at least one dimension")
+    return x.detach()
+
+
+def _kept(saved: Act8, what: str) -> Act8:
+    if not isinstance(saved, Act8):
+        raise TypeError(f"{what}: expected an Act8, got {type(saved).__name__}")
+    return saved
+
+
+def encode(x: torch.Tensor, fmt: str = "int8") -> Act8:
+    """x [..., d] (float32, bfloat16 or float16) in 8 bits."""
+    code = _fmt(fmt, "act8.encode")
+    x = _activation(x, "act8.encode")
+    rows = rows2d(x)
+    saved = Act8(x.shape, fmt, x.device)
+    codes, scales = saved._ptrs()
+    with on_device(rows):
+        _native._check(_native.lib().smx_act8_encode(
+            rows.data_ptr(), _native.dtype_code(rows.dtype), saved.rows, saved.cols, rows.stride(0), code, codes,
+            scales, saved.pitch, _native.stream_of(rows.device)), "smx_act8_encode")
+    return saved
+
+
+def decode(saved: Act8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The kept values in `dtype`: exact in bfloat16 and float32."""
+    _kept(saved, "act8.decode")
+    out = torch.empty(saved.shape, dtype=dtype, device=saved.data.device)
+    codes, scales = saved._ptrs()
+    with on_device(out):
+        _native._check(_native.lib().smx_act8_decode(
+            codes, scales, FORMATS[saved.fmt], saved.rows, saved.cols, saved.pitch, out.data_ptr(),
+            _native.dtype_code(dtype), saved.cols, _native.stream_of(out.device)), "smx_act8_decode")
+    return out
+
+
+def gelu_forward(h: torch.Tensor, fmt: str = "int8",
+                 keep_output: bool = True) -> Tuple[torch.Tensor, Act8, Optional[Act8]]:
+    """(GELU(h), h kept, the GELU's output kept or None) in one pass."""
+    code = _fmt(fmt, "act8.gelu_forward")
+    h = _activation(h, "act8.gelu_forward")
+    rows = rows2d(h)
+    y = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    kept_h = Act8(h.shape, fmt, h.device)
+    kept_y = Act8(h.shape, fmt, h.device) if keep_output else None
+    with on_device(rows):
+        _native._check(_native.lib().smx_act8_gelu(
+            rows.data_ptr(), _native.dtype_code(h.dtype), kept_h.rows, kept_h.cols, rows.stride(0), code, y.data_ptr(),
+            kept_h.cols, *kept_h._ptrs(), *(kept_y._ptrs() if keep_output else (None, None)), kept_h.pitch,
+            _native.stream_of(rows.device)), "smx_act8_gelu")
+    return y, kept_h, kept_y
+
+
+def gelu_backward(dy: torch.Tensor, saved: Act8) -> torch.Tensor:
+    """dy * GELU'(kept h), in dy's type."""
+    _kept(saved, "act8.gelu_backward")
+    dy = _activation(dy, "act8.gelu_backward")
+    if dy.shape != saved.shape:
+        raise ValueError(f"act8.gelu_backward: cotangent {tuple(dy.shape)} of a kept {tuple(saved.shape)}")
+    same_device("act8.gelu_backward", dy, saved.data)
+    rows = rows2d(dy)
+    dh = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    codes, scales = saved._ptrs()
+    with on_device(rows):
+        _native._check(_native.lib().smx_act8_gelu_backward(
+            rows.data_ptr(), _native.dtype_code(dy.dtype), saved.rows, saved.cols, rows.stride(0), codes, scales,
+            FORMATS[saved.fmt], saved.pitch, dh.data_ptr(), saved.cols, _native.stream_of(rows.device)),
+            "smx_act8_gelu_backward")
+    return dh
+
+
+def linear_backward(delta: torch.Tensor, saved: Act8, dtype: Optional[torch.dtype] = None,
+                    bias: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(dW [n, d], db [n] or None) of a Linear with output cotangent `delta`
+    [..., n] and kept input `saved` [..., d], in `dtype` (delta's by default),
+    each rounded once from FP32 sums."""
+    _kept(saved, "act8.linear_backward")
+    delta = _activation(delta, "act8.linear_backward")
+    if delta.shape[:-1] != saved.shape[:-1]:
+        raise ValueError(f"act8.linear_backward: cotangent {tuple(delta.shape)} of a kept input {tuple(saved.shape)}")
+    same_device("act8.linear_backward", delta, saved.data)
+    rows = rows2d(delta)
+    n = delta.shape[-1]
+    dtype = delta.dtype if dtype is None else dtype
+    out = _native.dtype_code(dtype)
+    code = _native.dtype_code(delta.dtype)
+    lib = _native.lib()
+    dw = torch.empty(n, saved.cols, dtype=dtype, device=delta.device)
+    db = torch.empty(n, dtype=dtype, device=delta.device) if bias else None
+    need = lib.smx_act8_wgrad_workspace_bytes(saved.rows, n, saved.cols, code)
+    work = torch.empty(need, dtype=torch.uint8, device=delta.device) if need else None
+    codes, scales = saved._ptrs()
+    with on_device(rows):
+        _native._check(lib.smx_act8_wgrad(
+            rows.data_ptr(), code, saved.rows, n, rows.stride(0), codes, scales, FORMATS[saved.fmt], saved.cols,
+            saved.pitch, dw.data_ptr(), _native.ptr(db), out, _native.ptr(work), need,
+            _native.stream_of(rows.device)), "smx_act8_wgrad")
+    return dw, db
+
+
+# ------------------------------------------------- differentiable functions ---
+def _cast(t: Optional[torch.Tensor], device_type: str) -> Optional[torch.Tensor]:
+    """t as autocast would hand it to a Linear."""
+    if t is None or not torch.is_autocast_enabled(device_type):
+        return t
+    return t.to(torch.get_autocast_dtype(device_type))
+
+
+def _input_grad(grad: torch.Tensor, weight: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    g2 = grad.reshape(-1, grad.shape[-1])
+    return g2.mm(weight).view(*grad.shape[:-1], weight.shape[1]).to(dtype)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, fmt):
+        x_lp, w, b = (_cast(t, x.device.type) for t in (x, weight, bias))
+        with torch.autocast(device_type=x.device.type, enabled=False):
+            y = F.linear(x_lp, w, b)
+        needs = ctx.needs_input_grad
+        ctx.kept = encode(x_lp, fmt) if needs[1] or needs[2] else None
+        ctx.save_for_backward(w)
+        ctx.dtypes = x.dtype, weight.dtype, None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        w, = ctx.saved_tensors
+        x_dtype, w_dtype, b_dtype = ctx.dtypes
+        needs = ctx.needs_input_grad
+        dx = _input_grad(grad, w, x_dtype) if needs[0] else None
+        dw = db = None
+        if needs[1] or needs[2]:
+            dw, db = linear_backward(grad, ctx.kept, w_dtype, bias=needs[2])
+            if db is not None and b_dtype != w_dtype:
+                db = db.to(b_dtype)
+        return dx, dw if needs[1] else None, db, None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+           fmt: str = "int8") -> torch.Tensor:
+    """F.linear whose input is kept in 8 bits for the weight gradient."""
+    need_float(x, "act8.linear")
+    _fmt(fmt, "act8.linear")
+    return _Linear.apply(x, weight, bias, fmt)
+
+
+class _Gelu(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, fmt):
+        y, ctx.kept, _ = gelu_forward(h, fmt, keep_output=False)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        return gelu_backward(grad, ctx.kept), None
+
+
+def gelu(h: torch.Tensor, fmt: str = "int8") -> torch.Tensor:
+    """F.gelu (exact form) whose input is kept in 8 bits."""
+    _fmt(fmt, "act8.gelu")
+    return _Gelu.apply(need_float(h, "act8.gelu"), fmt)
+
+
+class _Mlp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, fc_w, fc_b, proj_w, proj_b, fmt):
+        x_lp, w1, b1, w2, b2 = (_cast(t, x.device.type) for t in (x, fc_w, fc_b, proj_w, proj_b))
+        with torch.autocast(device_type=x.device.type, enabled=False):
+            ctx.kept_x = encode(x_lp, fmt)
+            y, ctx.kept_h, ctx.kept_y = gelu_forward(F.linear(x_lp, w1, b1), fmt)
+            out = F.linear(y, w2, b2)
+        ctx.save_for_backward(w1, w2)
+        ctx.dtypes = tuple(None if t is None else t.dtype for t in (x, fc_w, fc_b, proj_w, proj_b))
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        w1, w2 = ctx.saved_tensors
+        needs, types_ = ctx.needs_input_grad, ctx.dtypes
+        out = [None] * 6
+        if needs[3] or needs[4]:
+            out[3], out[4] = linear_backward(grad, ctx.kept_y, types_[3], bias=needs[4])
+        dh = gelu_backward(_input_grad(grad, w2, grad.dtype), ctx.kept_h)
+        if needs[1] or needs[2]:
+            out[1], out[2] = linear_backward(dh, ctx.kept_x, types_[1], bias=needs[2])
+        if needs[0]:
+            out[0] = _input_grad(dh, w1, types_[0])
+        for k in (2, 4):
+            if out[k] is not None and out[k].dtype != types_[k]:
+                out[k] = out[k].to(types_[k])
+        return tuple(g if k < 5 and needs[k] else None for k, g in enumerate(out))
+
+
+def mlp(x: torch.Tensor, fc_weight: torch.Tensor, fc_bias: Optional[torch.Tensor], proj_weight: torch.Tensor,
+        proj_bias: Optional[torch.Tensor], fmt: str = "int8") -> torch.Tensor:
+    """proj(GELU(fc(x))) with x, the hidden layer and the GELU's output kept in
+    8 bits: 1 byte an element where three 16-bit tensors would be kept."""
+    need_float(x, "act8.mlp")
+    _fmt(fmt, "act8.mlp")
+    return _Mlp.apply(x, fc_weight, fc_bias, proj_weight, proj_bias, fmt)
+
+
+class CheckpointedLinears:
+    """Handle of ``checkpoint_linears``; ``close()`` restores the forwards."""
+
+    def __init__(self, modules):
+        self.modules = modules
+
+    def close(self) -> None:
+        for module in self.modules.values():
+            module.__dict__.pop("forward", None)
+        self.modules = {}
+
+
+def checkpoint_linears(model: nn.Module, module_filter: Optional[Callable[[str, nn.Module], bool]] = None,
+                       fmt: str = "int8") -> CheckpointedLinears:
+    """Puts every plain ``nn.Linear`` of `model` that `module_filter` selects
+    (all of them by default) on ``linear``.  Hooks on the modules run as before;
+    a module whose forward is replaced already is left as it is."""
+    _fmt(fmt, "act8.checkpoint_linears")
+
+    def forward(module: nn.Linear, x: torch.Tensor) -> torch.Tensor:
+        if torch.is_grad_enabled() and x.device.type == "cuda":
+            return linear(x, module.weight, module.bias, fmt)
+        return F.linear(x, module.weight, module.bias)
+
+    chosen = {}
+    for name, module in model.named_modules():
+        if type(module) is not nn.Linear or "forward" in module.__dict__:
+            continue
+        if module_filter is None or module_filter(name, module):
+            module.forward = types.MethodType(forward, module)
+            chosen[name] = module
+    return CheckpointedLinears(chosen)

@@ -1,0 +1,310 @@
+// Activations kept in 8 bits for the backward pass (format: act8.h): encode,
+// decode, and the GELU of an MLP's hidden layer with its input and output
+// kept in the same pass.  All are one pass over the data, bound by HBM.
+//
+// A thread owns 8 neighbours of a row, so that a 16-bit row is read in 16-byte
+// loads, and four neighbouring lanes own a block of 32: the block's largest
+// magnitude is two DPP moves away.  blockDim = (chunks of 8, rows), so no
+// thread divides; each thread takes kRows rows, whose loads are all in flight
+// before the first is used.
+#include "act8.h"
+
+#include <algorithm>
+
+namespace smx {
+
+constexpr int kActRows = 4;
+
+template <int DT, bool VEC>
+struct Elems8 {
+  // Elements [i, i + n) of p, n <= 8; the rest are zero.
+  static __device__ __forceinline__ void load(const void *p, int64_t i, int n, float *v) {
+    if constexpr (VEC) {
+      if constexpr (DT == SMX_F32) {
+        const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+        const float4 b = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      } else {
+        const uint4 a = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (DT == SMX_BF16) {
+            v[2 * k] = __uint_as_float(w[k] << 16);
+            v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+          } else {
+            v[2 * k] = f16_bits_to_f32(static_cast<uint16_t>(w[k]));
+            v[2 * k + 1] = f16_bits_to_f32(static_cast<uint16_t>(w[k] >> 16));
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = k < n ? load_elem<DT>(p, i + k) : 0.f;
+    }
+  }
+  static __device__ __forceinline__ void store(void *p, int64_t i, int n, const float *v) {
+    if constexpr (VEC) {
+      if constexpr (DT == SMX_F32) {
+        float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(p) + i);
+        o[0] = make_float4(v[0], v[1], v[2], v[3]);
+        o[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (DT == SMX_BF16) {
+            w[k] = f32_to_bf16_bits(v[2 * k]) | (static_cast<uint32_t>(f32_to_bf16_bits(v[2 * k + 1])) << 16);
+          } else {
+            const _Float16 h[2] = {static_cast<_Float16>(v[2 * k]), static_cast<_Float16>(v[2 * k + 1])};
+            __builtin_memcpy(&w[k], h, 4);
+          }
+        }
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < n) store_any(p, DT, i + k, v[k]);
+    }
+  }
+};
+
+struct Act8Out {
+  uint8_t *codes;   // [rows, pitch]
+  uint8_t *scales;  // [rows, pitch / 32]
+};
+
+// Encodes 8 elements of every lane; `row`, `chunk` name them.
+template <int FMT>
+__device__ __forceinline__ void act8_put(const float *v, const Act8Out &o, int64_t row, int64_t pitch, int chunk) {
+  // Magnitudes compare as whole numbers, a NaN above all (fmaxf would drop it).
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+  top = max(top, dpp_mov<0xB1>(top));
+  top = max(top, dpp_mov<0x4E>(top));
+  const int b = act8_scale_byte<FMT>(static_cast<int>(top >> 23));
+  uint2 w = make_uint2(0, 0);
+  if (b != 255) {
+    const float inv = act8_scale(254 - b);
+    if (FMT == SMX_ACT8_E4M3 && (top >> 23) == 254) {
+      // (the code 128 of this scale would stand for 2^128)
+      float u[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u[k] = __builtin_amdgcn_fmed3f(v[k] * inv, -120.f, 120.f);
+      w = make_uint2(act8_pack4<FMT>(u, 1.f), act8_pack4<FMT>(u + 4, 1.f));
+    } else {
+      w = make_uint2(act8_pack4<FMT>(v, inv), act8_pack4<FMT>(v + 4, inv));
+    }
+  }
+  *reinterpret_cast<uint2 *>(o.codes + row * pitch + 8 * chunk) = w;
+  if ((chunk & 3) == 0) o.scales[row * (pitch >> 5) + (chunk >> 2)] = static_cast<uint8_t>(b);
+}
+
+struct Act8Args {
+  const void *x;
+  void *y;
+  const void *dy;
+  Act8Out x8, y8;
+  int64_t rows, cols, pitch, x_stride, y_stride, dy_stride;
+};
+
+// FP32 GELU in torch's order of operations: x * 0.5 * (1 + erf(x / sqrt 2)).
+__device__ __forceinline__ float act8_phi(float x) { return 0.5f * (1.f + erff(x * 0.70710678118654752f)); }
+
+enum Act8Op : int { kActEncode = 0, kActGelu = 1, kActDecode = 2, kActGeluBack = 3 };
+
+template <int DT, int FMT, int OP, bool VEC>
+__global__ void __launch_bounds__(256) act8_kernel(Act8Args a) {
+  using E = Elems8<DT, VEC>;
+  const int chunk = blockIdx.x * blockDim.x + threadIdx.x;
+  if (8 * static_cast<int64_t>(chunk) >= a.pitch) return;
+  const int n = static_cast<int>(min<int64_t>(8, max<int64_t>(0, a.cols - 8 * static_cast<int64_t>(chunk))));
+  const int64_t step = static_cast<int64_t>(gridDim.y) * blockDim.y;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; r0 < a.rows; r0 += step * kActRows) {
+    float v[kActRows][8];
+    uint2 codes[kActRows];
+    int b[kActRows];
+#pragma unroll
+    for (int u = 0; u < kActRows; ++u) {
+      const int64_t r = r0 + u * step;
+      if (r >= a.rows) break;
+      if constexpr (OP == kActEncode || OP == kActGelu) {
+        // (a vector load is whole or, in the padding, not made)
+        if (VEC && n == 0) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[u][k] = 0.f;
+        } else {
+          E::load(a.x, r * a.x_stride + 8 * chunk, n, v[u]);
+        }
+      } else {
+        codes[u] = *reinterpret_cast<const uint2 *>(a.x8.codes + r * a.pitch + 8 * chunk);
+        b[u] = a.x8.scales[r * (a.pitch >> 5) + (chunk >> 2)];
+        if (OP == kActGeluBack && n > 0) E::load(a.dy, r * a.dy_stride + 8 * chunk, n, v[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kActRows; ++u) {
+      const int64_t r = r0 + u * step;
+      if (r >= a.rows) break;
+      if constexpr (OP == kActEncode || OP == kActGelu) act8_put<FMT>(v[u], a.x8, r, a.pitch, chunk);
+      if constexpr (OP == kActGelu) {
+        // (the output is kept as it is stored: rounded to its type first)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[u][k] = round_to(DT, v[u][k] * act8_phi(v[u][k]));
+        if (n > 0) E::store(a.y, r * a.y_stride + 8 * chunk, n, v[u]);
+        if (a.y8.codes) act8_put<FMT>(v[u], a.y8, r, a.pitch, chunk);
+      }
+      if constexpr (OP == kActDecode || OP == kActGeluBack) {
+        if (n == 0) continue;
+        float h[8];
+        const float scale = act8_scale(b[u]);
+        act8_unpack4<FMT>(codes[u].x, scale, h);
+        act8_unpack4<FMT>(codes[u].y, scale, h + 4);
+        if constexpr (OP == kActGeluBack) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            h[k] = v[u][k] * (act8_phi(h[k]) + h[k] * (expf(-0.5f * h[k] * h[k]) * 0.3989422804014327f));
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[k] = round_to(DT, h[k]);
+        E::store(a.y, r * a.y_stride + 8 * chunk, n, h);
+      }
+    }
+  }
+}
+
+template <int DT, int FMT, int OP>
+static int act8_launch_as(const Act8Args &a, bool vec, hipStream_t st, const char *what) {
+  const int64_t chunks = a.pitch / 8;
+  const int64_t gx = ceil_div(chunks, 256);
+  const int tx = static_cast<int>(round_up(ceil_div(chunks, gx), 4));
+  const int ty = std::max(1, 256 / tx);
+  const int64_t gy = std::min<int64_t>(ceil_div(a.rows, static_cast<int64_t>(ty) * kActRows), 32768);
+  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), block(tx, ty);
+  if (vec) {
+    hipLaunchKernelGGL((act8_kernel<DT, FMT, OP, true>), grid, block, 0, st, a);
+  } else {
+    hipLaunchKernelGGL((act8_kernel<DT, FMT, OP, false>), grid, block, 0, st, a);
+  }
+  return check_launch(what);
+}
+
+template <int OP>
+static int act8_launch(const Act8Args &a, int dtype, int fmt, bool vec, hipStream_t st, const char *what) {
+  const bool i8 = fmt == SMX_ACT8_INT8;
+  if (dtype == SMX_F32)
+    return i8 ? act8_launch_as<SMX_F32, SMX_ACT8_INT8, OP>(a, vec, st, what)
+              : act8_launch_as<SMX_F32, SMX_ACT8_E4M3, OP>(a, vec, st, what);
+  if (dtype == SMX_BF16)
+    return i8 ? act8_launch_as<SMX_BF16, SMX_ACT8_INT8, OP>(a, vec, st, what)
+              : act8_launch_as<SMX_BF16, SMX_ACT8_E4M3, OP>(a, vec, st, what);
+  return i8 ? act8_launch_as<SMX_F16, SMX_ACT8_INT8, OP>(a, vec, st, what)
+            : act8_launch_as<SMX_F16, SMX_ACT8_E4M3, OP>(a, vec, st, what);
+}
+
+// 16-byte loads and stores of 8 elements: every row starts on 16 bytes and
+// holds whole groups of 8 (padding groups are not touched).
+static bool act8_vec(const void *p, int dtype, int64_t cols, int64_t stride, int64_t rows) {
+  const int64_t e = dtype == SMX_F32 ? 4 : 2;
+  return cols % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || stride * e % 16 == 0);
+}
+
+static std::string act8_name(const char *what, const char *msg) { return std::string(what) + ": " + msg; }
+
+static int act8_check(const char *what, int dtype, int fmt, int64_t rows, int64_t cols, int64_t pitch) {
+  SMX_REQUIRE(dtype == SMX_F32 || dtype == SMX_BF16 || dtype == SMX_F16, SMX_EDTYPE,
+              act8_name(what, "dtype must be f32, bf16 or f16"));
+  SMX_REQUIRE(fmt == SMX_ACT8_INT8 || fmt == SMX_ACT8_E4M3, SMX_EINVAL, act8_name(what, "unknown 8-bit format"));
+  SMX_REQUIRE(rows >= 0 && cols >= 0, SMX_ESHAPE, act8_name(what, "negative rows or cols"));
+  SMX_REQUIRE(cols <= (int64_t{1} << 30), SMX_ESHAPE, act8_name(what, "more than 2^30 columns"));
+  SMX_REQUIRE(pitch >= cols && pitch % kAct8Block == 0 && pitch - cols < kAct8Block, SMX_ESHAPE,
+              act8_name(what, "pitch must be cols rounded up to a multiple of 32"));
+  return SMX_OK;
+}
+
+static int act8_check_tensor(const char *what, const void *p, int64_t rows, int64_t cols, int64_t stride) {
+  SMX_REQUIRE(p, SMX_EINVAL, act8_name(what, "null pointer"));
+  SMX_REQUIRE(stride >= cols || rows <= 1, SMX_ESHAPE, act8_name(what, "row stride smaller than cols"));
+  return SMX_OK;
+}
+
+static int act8_check_codes(const char *what, const void *codes, const void *scales) {
+  SMX_REQUIRE(codes && scales, SMX_EINVAL, act8_name(what, "null codes or scales"));
+  SMX_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 16 == 0, SMX_EALIGN, act8_name(what, "codes must be 16-byte aligned"));
+  return SMX_OK;
+}
+
+}  // namespace smx
+
+using namespace smx;
+
+#define ACT8_TRY(call)           \
+  do {                           \
+    const int rc_ = (call);      \
+    if (rc_ != SMX_OK) return rc_; \
+  } while (0)
+
+extern "C" int smx_act8_encode(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int fmt,
+                               uint8_t *codes, uint8_t *scales, int64_t pitch, void *stream) {
+  const char *what = "act8_encode";
+  ACT8_TRY(act8_check(what, dtype, fmt, rows, cols, pitch));
+  if (rows == 0 || cols == 0) return SMX_OK;
+  ACT8_TRY(act8_check_tensor(what, x, rows, cols, row_stride));
+  ACT8_TRY(act8_check_codes(what, codes, scales));
+  Act8Args a{};
+  a.x = x, a.x8 = {codes, scales}, a.rows = rows, a.cols = cols, a.pitch = pitch, a.x_stride = row_stride;
+  return act8_launch<kActEncode>(a, dtype, fmt, act8_vec(x, dtype, cols, row_stride, rows),
+                                 static_cast<hipStream_t>(stream), what);
+}
+
+extern "C" int smx_act8_decode(const uint8_t *codes, const uint8_t *scales, int fmt, int64_t rows, int64_t cols,
+                               int64_t pitch, void *out, int dtype, int64_t out_stride, void *stream) {
+  const char *what = "act8_decode";
+  ACT8_TRY(act8_check(what, dtype, fmt, rows, cols, pitch));
+  if (rows == 0 || cols == 0) return SMX_OK;
+  ACT8_TRY(act8_check_tensor(what, out, rows, cols, out_stride));
+  ACT8_TRY(act8_check_codes(what, codes, scales));
+  Act8Args a{};
+  a.y = out, a.rows = rows, a.cols = cols, a.pitch = pitch, a.y_stride = out_stride;
+  a.x8 = {const_cast<uint8_t *>(codes), const_cast<uint8_t *>(scales)};
+  return act8_launch<kActDecode>(a, dtype, fmt, act8_vec(out, dtype, cols, out_stride, rows),
+                                 static_cast<hipStream_t>(stream), what);
+}
+
+extern "C" int smx_act8_gelu(const void *h, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int fmt, void *y,
+                             int64_t y_stride, uint8_t *h_codes, uint8_t *h_scales, uint8_t *y_codes,
+                             uint8_t *y_scales, int64_t pitch, void *stream) {
+  const char *what = "act8_gelu";
+  ACT8_TRY(act8_check(what, dtype, fmt, rows, cols, pitch));
+  if (rows == 0 || cols == 0) return SMX_OK;
+  ACT8_TRY(act8_check_tensor(what, h, rows, cols, row_stride));
+  ACT8_TRY(act8_check_tensor(what, y, rows, cols, y_stride));
+  ACT8_TRY(act8_check_codes(what, h_codes, h_scales));
+  SMX_REQUIRE((y_codes == nullptr) == (y_scales == nullptr), SMX_EINVAL,
+              "act8_gelu: the output's codes and scales must both be given or both be null");
+  if (y_codes) ACT8_TRY(act8_check_codes(what, y_codes, y_scales));
+  Act8Args a{};
+  a.x = h, a.y = y, a.x8 = {h_codes, h_scales}, a.y8 = {y_codes, y_scales};
+  a.rows = rows, a.cols = cols, a.pitch = pitch, a.x_stride = row_stride, a.y_stride = y_stride;
+  const bool vec = act8_vec(h, dtype, cols, row_stride, rows) && act8_vec(y, dtype, cols, y_stride, rows);
+  return act8_launch<kActGelu>(a, dtype, fmt, vec, static_cast<hipStream_t>(stream), what);
+}
+
+extern "C" int smx_act8_gelu_backward(const void *dy, int dtype, int64_t rows, int64_t cols, int64_t dy_stride,
+                                      const uint8_t *h_codes, const uint8_t *h_scales, int fmt, int64_t pitch,
+                                      void *dh, int64_t dh_stride, void *stream) {
+  const char *what = "act8_gelu_backward";
+  ACT8_TRY(act8_check(what, dtype, fmt, rows, cols, pitch));
+  if (rows == 0 || cols == 0) return SMX_OK;
+  ACT8_TRY(act8_check_tensor(what, dy, rows, cols, dy_stride));
+  ACT8_TRY(act8_check_tensor(what, dh, rows, cols, dh_stride));
+  ACT8_TRY(act8_check_codes(what, h_codes, h_scales));
+  Act8Args a{};
+  a.dy = dy, a.y = dh, a.x8 = {const_cast<uint8_t *>(h_codes), const_cast<uint8_t *>(h_scales)};
+  a.rows = rows, a.cols = cols, a.pitch = pitch, a.dy_stride = dy_stride, a.y_stride = dh_stride;
+  const bool vec = act8_vec(dy, dtype, cols, dy_stride, rows) && act8_vec(dh, dtype, cols, dh_stride, rows);
+  return act8_launch<kActGeluBack>(a, dtype, fmt, vec, static_cast<hipStream_t>(stream), what);
+}
