@@ -1,73 +1,381 @@
 // The weight and bias gradients of a Linear whose input is kept in 8 bits:
 //   dW[n, k] = sum_m delta[m, n] * held(x)[m, k],   db[n] = sum_m delta[m, n].
+//
+// One block of four waves owns a T x T tile of dW over a range of rows m (a
+// split) and goes over it in steps of kStep rows.  Both operands have the sum's
+// index m as their slow axis, so each step is staged row by row in LDS as BF16
+// and read back transposed (ds_read_b64_tr_b16: four rows of one column per
+// lane) as the operands of v_mfma_f32_32x32x16_bf16.  The codes become BF16 on
+// the way into LDS: a code times its scale is exact in BF16, so its product
+// with a BF16 cotangent is exact in FP32.  FP16 and FP32 cotangents are staged
+// as the two or three BF16 parts that sum to them exactly, with a product each.
+//
+// The two LDS buffers alternate: while one step's MFMAs run, the next step's
+// registers are written to the other and the loads of the step after are in
+// flight.  Splits of m write FP32 partial tiles that a second launch adds in
+// order, so the result does not depend on timing.
 #include "act8.h"
 
 #include <algorithm>
 
 namespace smx {
 
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
 struct WgradArgs {
   const void *delta;  // [rows, n] of its dtype
   const uint8_t *codes, *scales;
-  void *dw;  // [n, k]
-  void *db;  // [n] or null
+  void *dw;            // [n, k], or the splits' partial tiles [splits, n, k] in FP32
+  void *db;            // [n], or [splits, n] in FP32, or null
   int64_t rows, n, k, pitch, delta_stride;
+  int64_t split_rows;  // rows of a split, a multiple of the step
+  int32_t tiles_k, tiles, splits, out;
 };
 
-constexpr int kWgTile = 64, kWgStep = 16;
+constexpr int kWgThreads = 256;
+constexpr int parts_of(int dt) { return dt == SMX_BF16 ? 1 : dt == SMX_F16 ? 2 : 3; }
+// Rows of a step: its MFMAs (one product per part) cover the loads of the next.
+constexpr int wgrad_step(int dt, int tile) { return tile == 256 && dt != SMX_BF16 ? 32 : 64; }
 
-template <int DT, int FMT, int OUT>
-__global__ void __launch_bounds__(256) wgrad_kernel(WgradArgs a) {
-  __shared__ float sd[kWgStep][kWgTile], sx[kWgStep][kWgTile];
-  const int64_t n0 = static_cast<int64_t>(blockIdx.y) * kWgTile, k0 = static_cast<int64_t>(blockIdx.x) * kWgTile;
-  const int tn = threadIdx.x >> 4, tk = threadIdx.x & 15;
-  float acc[4][4] = {}, sum[4] = {};
-  for (int64_t m0 = 0; m0 < a.rows; m0 += kWgStep) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kWgStep * kWgTile; i += 256) {
-      const int r = i >> 6, c = i & 63;
-      const int64_t m = m0 + r;
-      sd[r][c] = m < a.rows && n0 + c < a.n ? load_elem<DT>(a.delta, m * a.delta_stride + n0 + c) : 0.f;
-      float x = 0.f;
-      if (m < a.rows && k0 + c < a.k) {
-        float v[4];
-        act8_unpack4<FMT>(a.codes[m * a.pitch + k0 + c], act8_scale(a.scales[m * (a.pitch >> 5) + ((k0 + c) >> 5)]), v);
-        x = v[0];
-      }
-      sx[r][c] = x;
+// 16 codes and their scale to 16 BF16 values (two uint4).
+template <int FMT>
+__device__ __forceinline__ void act8_to_bf16(const uint4 &c, int b, uint4 *o) {
+  const float scale = act8_scale(b);
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t r[8];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (FMT == SMX_ACT8_INT8) {
+      // (code + 128) scale - 128 scale, exact; the upper halves are the BF16 values
+      const uint32_t u = w[q] ^ 0x80808080u;
+      float f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        f[k] = fmaf(static_cast<float>((u >> (8 * k)) & 255u), scale, -128.f * scale);
+      r[2 * q] = __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u);
+      r[2 * q + 1] = __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u);
+    } else {
+      const v2bf lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[q], scale, false);
+      const v2bf hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[q], scale, true);
+      __builtin_memcpy(&r[2 * q], &lo, 4);
+      __builtin_memcpy(&r[2 * q + 1], &hi, 4);
     }
-    __syncthreads();
-    for (int r = 0; r < kWgStep; ++r) {
+  }
+  o[0] = make_uint4(r[0], r[1], r[2], r[3]);
+  o[1] = make_uint4(r[4], r[5], r[6], r[7]);
+}
+
+// Eight cotangents as loaded.
+template <int DT>
+struct Cot8 {
+  static constexpr int kWords = DT == SMX_F32 ? 8 : 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const void *p, int64_t i) {
+    // (16-byte loads at the elements' own alignment)
+    __builtin_memcpy(w, static_cast<const char *>(p) + i * (DT == SMX_F32 ? 4 : 2), sizeof(w));
+  }
+  __device__ __forceinline__ void load_some(const void *p, int64_t i, int n) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float d = sd[r][4 * tn + i];
-        sum[i] += d;
+    for (int k = 0; k < kWords; ++k) w[k] = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sx[r][4 * tk + j], acc[i][j]);
+    for (int k = 0; k < 8; ++k) {
+      if (k >= n) continue;
+      if constexpr (DT == SMX_F32) {
+        w[k] = static_cast<const uint32_t *>(p)[i + k];
+      } else {
+        w[k >> 1] |= static_cast<uint32_t>(static_cast<const uint16_t *>(p)[i + k]) << (16 * (k & 1));
       }
     }
   }
+  __device__ __forceinline__ float value(int k) const {
+    if constexpr (DT == SMX_F32) return __uint_as_float(w[k]);
+    if constexpr (DT == SMX_BF16) return __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
+    return f16_bits_to_f32(static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1))));
+  }
+  // Its BF16 parts: each the leading eight bits of what is left (exact), the
+  // rest of an infinity being nothing.
+  __device__ __forceinline__ void parts(uint4 *o) const {
+    if constexpr (DT == SMX_BF16) {
+      o[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      constexpr int P = parts_of(DT);
+      uint32_t r[P][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t n = n0 + 4 * tn + i;
-    if (n >= a.n) continue;
+      for (int q = 0; q < 4; ++q) {
+        float a = value(2 * q), b = value(2 * q + 1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t k = k0 + 4 * tk + j;
-      if (k < a.k) store_any(a.dw, OUT, n * a.k + k, round_to(OUT, acc[i][j]));
+        for (int p = 0; p < P; ++p) {
+          const uint32_t ua = __float_as_uint(a) & 0xffff0000u, ub = __float_as_uint(b) & 0xffff0000u;
+          r[p][q] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+          a = fabsf(a) == INFINITY ? 0.f : a - __uint_as_float(ua);
+          b = fabsf(b) == INFINITY ? 0.f : b - __uint_as_float(ub);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < P; ++p) o[p] = make_uint4(r[p][0], r[p][1], r[p][2], r[p][3]);
     }
-    if (a.db && blockIdx.x == 0 && tk == 0) store_any(a.db, OUT, n, round_to(OUT, sum[i]));
+  }
+};
+
+// LDS image of a step: [planes][kStep rows][T] BF16, where the 32-byte blocks
+// of a row are exchanged by its row number (block ^ 2 (row mod 4)): the four
+// rows that a transposing read takes from one column then lie in different banks.
+template <int T>
+__device__ __forceinline__ int lds_at(int row, int block) {
+  return row * 2 * T + ((block ^ ((row & 3) << 1)) << 5);
+}
+
+template <int DT, int FMT, int T>
+__global__ void __launch_bounds__(kWgThreads) wgrad_kernel(WgradArgs a) {
+  constexpr int P = parts_of(DT), kStep = wgrad_step(DT, T);
+  constexpr int kPlane = kStep * T * 2, kBuffer = (P + 1) * kPlane;
+  constexpr int kDeltaLoads = kStep * T / 8 / kWgThreads, kCodeLoads = kStep * T / 16 / kWgThreads;
+  constexpr int W = T / 2, F = W / 32;  // a wave's tile of W x W, in F x F MFMA tiles
+  __shared__ __attribute__((aligned(128))) char lds[2 * kBuffer];
+
+  // Blocks of one split run on one XCD as far as they can, since they share its rows.
+  const int64_t blocks = static_cast<int64_t>(a.tiles) * a.splits;
+  const int64_t share = (blocks + 7) / 8;
+  const int64_t id = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= share || id >= blocks) return;
+  const int split = static_cast<int>(id / a.tiles), tile = static_cast<int>(id % a.tiles);
+  const int64_t n0 = static_cast<int64_t>(tile / a.tiles_k) * T, k0 = static_cast<int64_t>(tile % a.tiles_k) * T;
+  const int64_t m_begin = split * a.split_rows, m_end = min(a.rows, m_begin + a.split_rows);
+  const int steps = static_cast<int>((m_end - m_begin + kStep - 1) / kStep);
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = (wave >> 1) * W, wk = (wave & 1) * W;
+
+  // Staging: a thread loads 8 cotangents (16 codes) of the same columns in
+  // every row of its own.  Columns past the end repeat others in bounds: what
+  // they add to is not stored.
+  const int d_row = tid / (T / 8), d_col = tid % (T / 8);
+  const int c_row = tid / (T / 16), c_col = tid % (T / 16);
+  const int64_t nc = min(n0 + 8 * d_col, (a.n - 1) & ~int64_t{7});
+  const int nc_count = static_cast<int>(min<int64_t>(8, a.n - nc));
+  const int64_t kc = min(k0 + 16 * c_col, a.pitch - 16);
+  const int64_t scale_pitch = a.pitch >> 5;
+
+  Cot8<DT> d[kDeltaLoads];
+  uint4 c[kCodeLoads];
+  int s[kCodeLoads];
+  float sum[8] = {};
+  const bool bias = a.db && k0 == 0;
+
+  const auto load = [&](int step) __attribute__((always_inline)) {
+    const int64_t m0 = m_begin + static_cast<int64_t>(step) * kStep;
+    // A load of 8 that begins in a row may end in the next: the tensor's last
+    // row, and rows shorter than 8, are read one by one.  (No inputs, k = 0,
+    // leave no codes to read.)
+    if (m0 + kStep < a.rows && m0 + kStep <= m_end && a.n >= 8 && a.k > 0) {
+#pragma unroll
+      for (int i = 0; i < kDeltaLoads; ++i)
+        d[i].load(a.delta, (m0 + d_row + i * (kStep / kDeltaLoads)) * a.delta_stride + nc);
+#pragma unroll
+      for (int i = 0; i < kCodeLoads; ++i) {
+        const int64_t m = m0 + c_row + i * (kStep / kCodeLoads);
+        c[i] = *reinterpret_cast<const uint4 *>(a.codes + m * a.pitch + kc);
+        s[i] = a.scales[m * scale_pitch + (kc >> 5)];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kDeltaLoads; ++i) {
+        const int64_t m = m0 + d_row + i * (kStep / kDeltaLoads);
+        d[i].load_some(a.delta, m * a.delta_stride + nc, m < m_end ? nc_count : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kCodeLoads; ++i) {
+        const int64_t m = m0 + c_row + i * (kStep / kCodeLoads);
+        c[i] = make_uint4(0, 0, 0, 0);
+        s[i] = 1;
+        if (m < m_end && a.k > 0) {
+          c[i] = *reinterpret_cast<const uint4 *>(a.codes + m * a.pitch + kc);
+          s[i] = a.scales[m * scale_pitch + (kc >> 5)];
+        }
+      }
+    }
+  };
+  const auto stage = [&](int buffer) __attribute__((always_inline)) {
+    char *at = lds + buffer * kBuffer;
+#pragma unroll
+    for (int i = 0; i < kDeltaLoads; ++i) {
+      const int row = d_row + i * (kStep / kDeltaLoads);
+      uint4 o[P];
+      d[i].parts(o);
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        *reinterpret_cast<uint4 *>(at + p * kPlane + lds_at<T>(row, d_col >> 1) + (d_col & 1) * 16) = o[p];
+    }
+    if (bias) {
+#pragma unroll
+      for (int i = 0; i < kDeltaLoads; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] += d[i].value(k);
+    }
+#pragma unroll
+    for (int i = 0; i < kCodeLoads; ++i) {
+      const int row = c_row + i * (kStep / kCodeLoads);
+      uint4 o[2];
+      act8_to_bf16<FMT>(c[i], s[i], o);
+      uint4 *to = reinterpret_cast<uint4 *>(at + P * kPlane + lds_at<T>(row, c_col));
+      to[0] = o[0], to[1] = o[1];
+    }
+  };
+
+  // Transposing reads: lane i of a group of 16 names four columns of row
+  // i / 4 and receives column i of four rows; groups 0 and 1 hold columns 0-15
+  // and 16-31 of rows 0-7 of a 16-row operand, groups 2 and 3 rows 8-15.
+  const int g = lane >> 4, i16 = lane & 15, r4 = i16 >> 2;
+  int a_at[F], b_at[F];
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    const int row = 8 * (g >> 1) + r4;
+    a_at[f] = lds_at<T>(row, (wn >> 4) + 2 * f + (g & 1)) + (i16 & 3) * 8;
+    b_at[f] = lds_at<T>(row, (wk >> 4) + 2 * f + (g & 1)) + (i16 & 3) * 8;
+  }
+  const auto operand = [&](const char *at) __attribute__((always_inline)) {
+    typedef __attribute__((address_space(3))) v4s *lds_ptr;
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at));
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 4 * 2 * T));
+    typedef short v8s __attribute__((ext_vector_type(8)));
+    const v8s v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(v8bf, v);
+  };
+
+  v16f acc[F][F] = {};
+  if (steps > 0) {
+    load(0);
+    stage(0);
+  }
+  __syncthreads();
+  for (int t = 0; t < steps; ++t) {
+    if (t + 1 < steps) load(t + 1);
+    const char *at = lds + (t & 1) * kBuffer;
+#pragma unroll
+    for (int ms = 0; ms < kStep / 16; ++ms) {
+      v8bf bv[F];
+#pragma unroll
+      for (int f = 0; f < F; ++f) bv[f] = operand(at + P * kPlane + ms * 16 * 2 * T + b_at[f]);
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+          const v8bf av = operand(at + p * kPlane + ms * 16 * 2 * T + a_at[f]);
+#pragma unroll
+          for (int h = 0; h < F; ++h) acc[f][h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av, bv[h], acc[f][h], 0, 0, 0);
+        }
+    }
+    if (t + 1 < steps) stage((t & 1) ^ 1);
+    __syncthreads();
+  }
+
+  // Lane l holds column l mod 32 and rows 8 (r / 4) + 4 (l / 32) + r mod 4: an
+  // offset of the lane's own, from addresses that the wave shares.
+  const auto each = [&](auto store) __attribute__((always_inline)) {
+    const int64_t nb = n0 + wn, kb = k0 + wk;
+    const int ln = 4 * (lane >> 5), lk = lane & 31;
+    const uint32_t off = static_cast<uint32_t>(ln) * static_cast<uint32_t>(a.k) + lk;
+    const bool inside = nb + W <= a.n && kb + W <= a.k;
+    int64_t at = (a.splits > 1 ? static_cast<int64_t>(split) * a.n * a.k : 0) + nb * a.k + kb;
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = 32 * f + 8 * (r >> 2) + (r & 3);
+#pragma unroll
+        for (int h = 0; h < F; ++h) {
+          float v = acc[f][h][r];
+          // (keeps the compiler from moving every sum and address at once)
+          asm volatile("" : "+s"(at), "+v"(v));
+          if (inside || (nb + row + ln < a.n && kb + 32 * h + lk < a.k)) store(at + 32 * h, off, v);
+        }
+        at += (r & 3) == 3 ? 5 * a.k : a.k;
+      }
+  };
+  if (a.out == SMX_F32) {
+    each([&](int64_t i, uint32_t o, float v) __attribute__((always_inline)) { (static_cast<float *>(a.dw) + i)[o] = v; });
+  } else {
+    each([&](int64_t i, uint32_t o, float v) __attribute__((always_inline)) {
+      const _Float16 half = static_cast<_Float16>(v);
+      (static_cast<uint16_t *>(a.dw) + i)[o] = a.out == SMX_BF16 ? f32_to_bf16_bits(v) : __builtin_bit_cast(uint16_t, half);
+    });
+  }
+  if (bias) {
+    float *red = reinterpret_cast<float *>(lds);  // [rows of threads][T]
+#pragma unroll
+    for (int k = 0; k < 8; ++k) red[d_row * T + 8 * d_col + k] = sum[k];
+    __syncthreads();
+    if (tid < T && n0 + tid < a.n) {
+      float t = 0.f;
+      for (int q = 0; q < kWgThreads / (T / 8); ++q) t += red[q * T + tid];
+      store_any(a.db, a.out, (a.splits > 1 ? split * a.n : 0) + n0 + tid, round_to(a.out, t));
+    }
   }
 }
 
-template <int DT, int FMT>
-static void wgrad_launch(const WgradArgs &a, int out, dim3 grid, hipStream_t st) {
-  if (out == SMX_F32) {
-    hipLaunchKernelGGL((wgrad_kernel<DT, FMT, SMX_F32>), grid, dim3(256), 0, st, a);
-  } else if (out == SMX_BF16) {
-    hipLaunchKernelGGL((wgrad_kernel<DT, FMT, SMX_BF16>), grid, dim3(256), 0, st, a);
+// The splits' partial sums added in order.
+__global__ void __launch_bounds__(256) wgrad_join_kernel(const float *part, int64_t count, int splits, void *out,
+                                                         int out_dtype, const float *part_db, int64_t n, void *db) {
+  const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i0 + 4 <= count && count % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+    float4 t = make_float4(0, 0, 0, 0);
+    for (int s = 0; s < splits; ++s) {
+      const float4 v = *reinterpret_cast<const float4 *>(part + s * count + i0);
+      t.x += v.x, t.y += v.y, t.z += v.z, t.w += v.w;
+    }
+    if (out_dtype == SMX_F32) {
+      *reinterpret_cast<float4 *>(static_cast<float *>(out) + i0) = t;
+    } else {
+      store_any(out, out_dtype, i0, round_to(out_dtype, t.x));
+      store_any(out, out_dtype, i0 + 1, round_to(out_dtype, t.y));
+      store_any(out, out_dtype, i0 + 2, round_to(out_dtype, t.z));
+      store_any(out, out_dtype, i0 + 3, round_to(out_dtype, t.w));
+    }
   } else {
-    hipLaunchKernelGGL((wgrad_kernel<DT, FMT, SMX_F16>), grid, dim3(256), 0, st, a);
+    for (int64_t i = i0; i < min(i0 + 4, count); ++i) {
+      float t = 0.f;
+      for (int s = 0; s < splits; ++s) t += part[s * count + i];
+      store_any(out, out_dtype, i, round_to(out_dtype, t));
+    }
+  }
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (db && j < n) {
+    float t = 0.f;
+    for (int s = 0; s < splits; ++s) t += part_db[s * n + j];
+    store_any(db, out_dtype, j, round_to(out_dtype, t));
+  }
+}
+
+struct WgradPlan {
+  int tile, tiles_n, tiles_k, splits;
+  int64_t split_rows;
+};
+
+// 256 x 256 tiles (one block per CU) where they fill the CUs with few splits;
+// 128 x 128 tiles (two blocks per CU) otherwise.
+static WgradPlan wgrad_plan(int dtype, int64_t rows, int64_t n, int64_t k) {
+  WgradPlan p{};
+  constexpr int64_t kCus = 256;
+  p.tile = ceil_div(n, 256) * ceil_div(k, 256) * 4 >= kCus ? 256 : 128;
+  p.tiles_n = static_cast<int>(ceil_div(n, p.tile)), p.tiles_k = static_cast<int>(std::max<int64_t>(1, ceil_div(k, p.tile)));
+  const int64_t step = wgrad_step(dtype, p.tile), tiles = static_cast<int64_t>(p.tiles_n) * p.tiles_k;
+  const int64_t slots = kCus * (p.tile == 256 ? 1 : 2);
+  int64_t splits = std::max<int64_t>(1, slots / tiles);
+  splits = std::min(splits, std::max<int64_t>(1, rows / (4 * step)));
+  p.split_rows = round_up(ceil_div(std::max<int64_t>(rows, 1), splits), step);
+  p.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(rows, p.split_rows)));
+  return p;
+}
+
+template <int DT, int FMT>
+static void wgrad_launch(const WgradArgs &a, int tile, dim3 grid, hipStream_t st) {
+  if (tile == 256) {
+    hipLaunchKernelGGL((wgrad_kernel<DT, FMT, 256>), grid, dim3(kWgThreads), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((wgrad_kernel<DT, FMT, 128>), grid, dim3(kWgThreads), 0, st, a);
   }
 }
 
@@ -77,7 +385,8 @@ using namespace smx;
 
 extern "C" int64_t smx_act8_wgrad_workspace_bytes(int64_t rows, int64_t n, int64_t k, int dtype) {
   if (rows < 0 || n < 0 || k < 0 || dtype < SMX_F32 || dtype > SMX_F16) return SMX_EINVAL;
-  return 0;
+  const WgradPlan p = wgrad_plan(dtype, rows, n, k);
+  return p.splits == 1 ? 0 : round_up(p.splits * (n * k + n) * static_cast<int64_t>(sizeof(float)), 256);
 }
 
 extern "C" int smx_act8_wgrad(const void *delta, int dtype, int64_t rows, int64_t n, int64_t delta_stride,
@@ -99,20 +408,35 @@ extern "C" int smx_act8_wgrad(const void *delta, int dtype, int64_t rows, int64_
   }
   const int64_t need = smx_act8_wgrad_workspace_bytes(rows, n, k, dtype);
   SMX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), SMX_EWORKSPACE, "act8_wgrad: workspace too small");
-  const WgradArgs a{delta, codes, scales, dw, db, rows, n, k, pitch, delta_stride};
-  const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, ceil_div(k, kWgTile))),
-                  static_cast<unsigned>(ceil_div(n, kWgTile)));
+  SMX_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 256 == 0, SMX_EALIGN,
+              "act8_wgrad: workspace must be 256-byte aligned");
+  const WgradPlan p = wgrad_plan(dtype, rows, n, k);
+  WgradArgs a{};
+  a.delta = delta, a.codes = codes, a.scales = scales, a.dw = dw, a.db = db;
+  a.rows = rows, a.n = n, a.k = k, a.pitch = pitch, a.delta_stride = delta_stride;
+  a.split_rows = p.split_rows, a.tiles_k = p.tiles_k, a.tiles = p.tiles_n * p.tiles_k, a.splits = p.splits, a.out = out_dtype;
+  if (p.splits > 1) {
+    a.dw = workspace, a.out = SMX_F32;
+    if (db) a.db = static_cast<float *>(workspace) + p.splits * n * k;
+  }
+  const dim3 grid(static_cast<unsigned>(round_up(static_cast<int64_t>(a.tiles) * a.splits, 8)));
   const auto st = static_cast<hipStream_t>(stream);
   const bool i8 = fmt == SMX_ACT8_INT8;
   if (dtype == SMX_F32) {
-    i8 ? wgrad_launch<SMX_F32, SMX_ACT8_INT8>(a, out_dtype, grid, st)
-       : wgrad_launch<SMX_F32, SMX_ACT8_E4M3>(a, out_dtype, grid, st);
+    i8 ? wgrad_launch<SMX_F32, SMX_ACT8_INT8>(a, p.tile, grid, st) : wgrad_launch<SMX_F32, SMX_ACT8_E4M3>(a, p.tile, grid, st);
   } else if (dtype == SMX_BF16) {
-    i8 ? wgrad_launch<SMX_BF16, SMX_ACT8_INT8>(a, out_dtype, grid, st)
-       : wgrad_launch<SMX_BF16, SMX_ACT8_E4M3>(a, out_dtype, grid, st);
+    i8 ? wgrad_launch<SMX_BF16, SMX_ACT8_INT8>(a, p.tile, grid, st)
+       : wgrad_launch<SMX_BF16, SMX_ACT8_E4M3>(a, p.tile, grid, st);
   } else {
-    i8 ? wgrad_launch<SMX_F16, SMX_ACT8_INT8>(a, out_dtype, grid, st)
-       : wgrad_launch<SMX_F16, SMX_ACT8_E4M3>(a, out_dtype, grid, st);
+    i8 ? wgrad_launch<SMX_F16, SMX_ACT8_INT8>(a, p.tile, grid, st) : wgrad_launch<SMX_F16, SMX_ACT8_E4M3>(a, p.tile, grid, st);
+  }
+  if (p.splits > 1) {
+    const int rc = check_launch("act8_wgrad");
+    if (rc != SMX_OK) return rc;
+    const int64_t count = n * k;
+    hipLaunchKernelGGL(wgrad_join_kernel, dim3(static_cast<unsigned>(std::max(ceil_div(count, 1024), ceil_div(n, 256)))),
+                       dim3(256), 0, st, static_cast<const float *>(workspace), count, p.splits, dw, out_dtype,
+                       static_cast<const float *>(a.db), n, db);
   }
   return check_launch("act8_wgrad");
 }
