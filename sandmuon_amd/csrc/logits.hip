@@ -19,80 +19,285 @@ struct LogitRows {
   int64_t batch, seq, vocab, batch_stride, row_stride;
 };
 
-constexpr int kRowThreads = 256;
+// ------------------------------------------------------------- one row ---
+// A row is held in registers from its one read to its gradient's one write:
+// NT threads with up to NCH 16-byte chunks each, all of whose loads are in
+// flight at once.  Chunks begin at the row's first element, at the elements'
+// own alignment (an odd vocabulary moves every row's start), so the sums do
+// not depend on where a row lies; the elements behind the last whole chunk
+// are one of each of the first threads.
+typedef uint32_t v4u_any __attribute__((ext_vector_type(4), aligned(2)));
 
-__device__ __forceinline__ float block_max(float v, float *scratch) {
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-  __syncthreads();
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 6); ++w) v = fmaxf(v, scratch[w]);
-  return v;
-}
-
-struct RowLp {
-  float top, sum;  // lse = top + log(sum)
-  float lp;
+template <int DT>
+struct Logit {
+  static constexpr int kBytes = DT == SMX_F32 ? 4 : 2, kPer = 16 / kBytes;  // elements of a chunk
+  static constexpr uint32_t kNone = DT == SMX_F32 ? 0xff800000u : DT == SMX_BF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
+  static __device__ __forceinline__ float at(const uint4 &c, int k) {
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    if constexpr (DT == SMX_F32) return __uint_as_float(w[k]);
+    if constexpr (DT == SMX_BF16) return __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
+    return f16_bits_to_f32(static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1))));
+  }
+  static __device__ __forceinline__ uint4 pack(const float *v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (DT == SMX_F32) {
+        w[k] = __float_as_uint(v[k]);
+      } else if constexpr (DT == SMX_BF16) {
+        typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+        const v2bf h = {static_cast<__bf16>(v[2 * k]), static_cast<__bf16>(v[2 * k + 1])};
+        __builtin_memcpy(&w[k], &h, 4);
+      } else {
+        const _Float16 h[2] = {static_cast<_Float16>(v[2 * k]), static_cast<_Float16>(v[2 * k + 1])};
+        __builtin_memcpy(&w[k], h, 4);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
 };
 
+// exp(d) for d <= 0.  16-bit logits: exp2 of the rounded product, within 2^-23
+// per unit of d; FP32 ones: the product's rounding made good.
 template <int DT>
-__device__ __forceinline__ RowLp row_lp(const LogitRows &a, int64_t at, int64_t y, float *scratch) {
-  float top = -INFINITY;
-  for (int64_t v = threadIdx.x; v < a.vocab; v += kRowThreads) top = fmaxf(top, load_elem<DT>(a.z, at + v));
-  top = block_max(top, scratch);
-  float sum = 0.f;
-  for (int64_t v = threadIdx.x; v < a.vocab; v += kRowThreads) sum += expf(load_elem<DT>(a.z, at + v) - top);
-  sum = block_sum(sum, scratch);
-  const double z = y >= 0 && y < a.vocab ? static_cast<double>(load_elem<DT>(a.z, at + y)) : __builtin_nan("");
-  return {top, sum, static_cast<float>((z - top) - log(static_cast<double>(sum)))};
+__device__ __forceinline__ float exp_of(float d) {
+  const float t = d * 1.44269504088896341f;
+  const float e = __builtin_amdgcn_exp2f(t);
+  if constexpr (DT != SMX_F32) return e;
+  const float rest = fmaf(d, 1.92596299112661e-8f, fmaf(d, 1.44269504088896341f, -t));
+  // (an infinite d has no rest)
+  return t > -200.f ? fmaf(e, 0.6931471805599453f * rest, e) : e;
 }
 
-// out[v] = c (onehot(y) - p).
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dpp_mov<0xB1>(v));
+  v = fmaxf(v, dpp_mov<0x4E>(v));
+  v = fmaxf(v, dpp_mov<0x141>(v));
+  v = fmaxf(v, dpp_mov<0x140>(v));
+  return fmaxf(fmaxf(read_lane(v, 0), read_lane(v, 16)), fmaxf(read_lane(v, 32), read_lane(v, 48)));
+}
+
+// What is left of sum * exp(m - top) where m may be top itself, infinite or not.
 template <int DT>
-__device__ __forceinline__ void row_grad(const LogitRows &a, int64_t at, int64_t y, float top, float sum, float c,
-                                         void *out, int64_t out_at) {
-  const float inv = 1.f / sum;
-  for (int64_t v = threadIdx.x; v < a.vocab; v += kRowThreads) {
-    const float p = expf(load_elem<DT>(a.z, at + v) - top) * inv;
-    store_any(out, DT, out_at + v, round_to(DT, v == y ? c - c * p : -c * p));
+__device__ __forceinline__ float moved(float sum, float m, float top) {
+  return m == top ? sum : sum * exp_of<DT>(m - top);
+}
+
+struct RowStat {
+  float top, sum;  // lse = top + log(sum)
+};
+
+template <int DT, int NT, int NCH>
+struct Row {
+  using L = Logit<DT>;
+  uint4 c[NCH];
+  float edge;   // this thread's element behind the whole chunks
+  int edge_at;  // its place, or -1
+  int chunks;   // whole chunks
+  int tid;
+  const char *src;
+
+  __device__ __forceinline__ void load(const void *z, int64_t at, int64_t vocab) {
+    const char *row = src = static_cast<const char *>(z) + at * L::kBytes;
+    tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
+    const int v = static_cast<int>(vocab);
+    chunks = v / L::kPer;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      c[i] = make_uint4(L::kNone, L::kNone, L::kNone, L::kNone);
+      if (i * NT < chunks && tid + i * NT < chunks) {
+        const v4u_any w = __builtin_nontemporal_load(reinterpret_cast<const v4u_any *>(row) + tid + i * NT);
+        c[i] = make_uint4(w.x, w.y, w.z, w.w);
+      }
+    }
+    edge_at = tid < v - chunks * L::kPer ? chunks * L::kPer + tid : -1;
+    edge = edge_at >= 0 ? load_elem<DT>(row, edge_at) : -INFINITY;
   }
+
+  __device__ __forceinline__ RowStat stat(float2 *scratch) const {
+    float m = edge;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      if (i * NT >= chunks) break;
+#pragma unroll
+      for (int k = 0; k < L::kPer; ++k) m = fmaxf(m, L::at(c[i], k));
+    }
+    // (a thread whose elements are all -inf adds nothing)
+    const float from = m == -INFINITY ? 0.f : m;
+    float s = exp_of<DT>(edge - from);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      if (i * NT >= chunks) break;
+#pragma unroll
+      for (int k = 0; k < L::kPer; ++k) s += exp_of<DT>(L::at(c[i], k) - from);
+    }
+    RowStat r;
+    r.top = wave_max(m);
+    r.sum = wave_sum(moved<DT>(s, m, r.top));
+    if constexpr (NT > 64) {
+      if ((tid & 63) == 0) scratch[tid >> 6] = make_float2(r.top, r.sum);
+      __syncthreads();
+      float2 w[NT / 64];
+      float top = -INFINITY;
+#pragma unroll
+      for (int q = 0; q < NT / 64; ++q) {
+        w[q] = scratch[q];
+        top = fmaxf(top, w[q].x);
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < NT / 64; ++q) sum += moved<DT>(w[q].y, w[q].x, top);
+      r.top = top, r.sum = sum;
+    }
+    return r;
+  }
+
+  // out[v] = c (onehot(y) - p)
+  __device__ __forceinline__ void grad(void *out, int64_t at, int64_t y, const RowStat &r, float coef) const {
+    char *row = static_cast<char *>(out) + at * L::kBytes;
+    const float scale = -coef / r.sum;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      if (i * NT >= chunks) break;
+      if (tid + i * NT < chunks) {
+        float v[L::kPer];
+#pragma unroll
+        for (int k = 0; k < L::kPer; ++k) v[k] = exp_of<DT>(L::at(c[i], k) - r.top) * scale;
+        put(row, i, L::pack(v));
+      }
+    }
+    if (edge_at >= 0) store_any(row, DT, edge_at, round_to(DT, exp_of<DT>(edge - r.top) * scale));
+    // the target's element again, by the thread that wrote it
+    const int t = static_cast<int>(y);
+    const bool mine = t >= chunks * L::kPer ? t == edge_at : tid == t / L::kPer % NT;
+    if (y >= 0 && mine)
+      store_any(row, DT, y, round_to(DT, fmaf(exp_of<DT>(load_elem<DT>(src, y) - r.top), scale, coef)));
+  }
+
+  __device__ __forceinline__ void zero(void *out, int64_t at, int64_t vocab) {
+    char *row = static_cast<char *>(out) + at * L::kBytes;
+    tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
+    const int v = static_cast<int>(vocab);
+    chunks = v / L::kPer;
+    for (int i = 0; i * NT < chunks; ++i)
+      if (tid + i * NT < chunks) put(row, i, make_uint4(0, 0, 0, 0));
+    if (tid < v - chunks * L::kPer) store_any(row, DT, chunks * L::kPer + tid, 0.f);
+  }
+
+  __device__ __forceinline__ void put(char *row, int i, const uint4 &w) const {
+    __builtin_nontemporal_store(v4u_any{w.x, w.y, w.z, w.w}, reinterpret_cast<v4u_any *>(row) + tid + i * NT);
+  }
+};
+
+// A row of any length, read again for each use: first the maximum and sum,
+// then the gradient.
+template <int DT>
+struct LongRow {
+  static constexpr int NT = 1024;
+  const void *z;
+  int64_t at, vocab;
+  __device__ __forceinline__ void load(const void *p, int64_t i, int64_t v) { z = p, at = i, vocab = v; }
+  __device__ __forceinline__ RowStat stat(float2 *scratch) const {
+    float m = -INFINITY, s = 0.f;
+    for (int64_t v = threadIdx.x; v < vocab; v += NT) {
+      const float x = load_elem<DT>(z, at + v);
+      const float top = fmaxf(m, x), from = top == -INFINITY ? 0.f : top;
+      s = moved<DT>(s, m, top) + exp_of<DT>(x - from);
+      m = top;
+    }
+    RowStat r;
+    r.top = wave_max(m);
+    r.sum = wave_sum(moved<DT>(s, m, r.top));
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = make_float2(r.top, r.sum);
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f;
+    for (int q = 0; q < NT / 64; ++q) top = fmaxf(top, scratch[q].x);
+    for (int q = 0; q < NT / 64; ++q) sum += moved<DT>(scratch[q].y, scratch[q].x, top);
+    return {top, sum};
+  }
+  __device__ __forceinline__ void grad(void *out, int64_t o, int64_t y, const RowStat &r, float coef) const {
+    const float scale = -coef / r.sum;
+    for (int64_t v = threadIdx.x; v < vocab; v += NT) {
+      const float e = exp_of<DT>(load_elem<DT>(z, at + v) - r.top);
+      store_any(out, DT, o + v, round_to(DT, v == y ? fmaf(e, scale, coef) : e * scale));
+    }
+  }
+  __device__ __forceinline__ void zero(void *out, int64_t o, int64_t v) const {
+    for (int64_t i = threadIdx.x; i < v; i += NT) store_any(out, DT, o + i, 0.f);
+  }
+};
+
+// Rows of a block and this thread's one; -1 where there is none.
+template <int NT>
+__device__ __forceinline__ int64_t row_of(int64_t rows) {
+  if constexpr (NT > 64) return blockIdx.x;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  return r < rows ? r : -1;
 }
 
+// z_y - lse.  The logarithm as its exponent's part and its fraction's, so that
+// only the result is rounded.
 template <int DT>
-__device__ __forceinline__ void row_zero(void *out, int64_t out_at, int64_t vocab) {
-  for (int64_t v = threadIdx.x; v < vocab; v += kRowThreads) store_any(out, DT, out_at + v, 0.f);
+__device__ __forceinline__ float target_lp(const LogitRows &a, int64_t at, int64_t y, const RowStat &r) {
+  const float z = y >= 0 && y < a.vocab ? load_elem<DT>(a.z, at + y) : __builtin_nanf("");
+  int e;
+  float m = frexpf(r.sum, &e);
+  if (m < 0.70710678f) m *= 2.f, --e;
+  const float hi = static_cast<float>(e) * 0.693145751953125f;  // (15 bits of log 2: exact)
+  const float lo = fmaf(static_cast<float>(e), 1.4286068203094172e-6f, logf(m));
+  return ((z - r.top) - hi) - lo;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kRowThreads) logprob_kernel(LogitRows a, float *logprobs, float2 *stats) {
-  __shared__ float scratch[16];
-  const int64_t r = blockIdx.x;
+// The row kernels' form of a vocabulary: threads and chunks a row.
+#define ROW_KERNEL(R, NT, NAME, ...) \
+  template <int DT, class R, int NT>  \
+  __global__ void __launch_bounds__(NT == 64 ? 256 : NT) NAME(__VA_ARGS__)
+
+ROW_KERNEL(R, NT, logprob_kernel, LogitRows a, float *logprobs, float2 *stats) {
+  __shared__ float2 scratch[16];
+  const int64_t r = row_of<NT>(a.batch * a.seq);
+  if (r < 0) return;
+  const int lane = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
   if (a.mask && !a.mask[r]) {
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
       logprobs[r] = 0.f;
       if (stats) stats[r] = make_float2(0.f, 1.f);
     }
     return;
   }
-  const RowLp o = row_lp<DT>(a, r / a.seq * a.batch_stride + r % a.seq * a.row_stride, a.targets[r], scratch);
-  if (threadIdx.x == 0) {
-    logprobs[r] = o.lp;
+  const int64_t at = r / a.seq * a.batch_stride + r % a.seq * a.row_stride, y = a.targets[r];
+  R row;
+  row.load(a.z, at, a.vocab);
+  const RowStat o = row.stat(scratch);
+  const float lp = target_lp<DT>(a, at, y, o);
+  if (lane == 0) {
+    logprobs[r] = lp;
     if (stats) stats[r] = make_float2(o.top, o.sum);
   }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kRowThreads) logprob_back_kernel(LogitRows a, const float2 *stats, const float *coef,
-                                                                   int64_t coef_batch, int64_t coef_seq,
-                                                                   const float *scale, void *dz) {
-  const int64_t r = blockIdx.x, b = r / a.seq, t = r % a.seq;
-  const bool live = !a.mask || a.mask[r];
-  if (!live) return row_zero<DT>(dz, r * a.vocab, a.vocab);
-  float c = coef[b * coef_batch + t * coef_seq];
-  if (scale) c *= *scale;
+struct CoefArgs {
+  const float2 *stats;
+  const float *coef, *scale;
+  int64_t batch_stride, row_stride;
+  void *dz;
+};
+
+ROW_KERNEL(R, NT, logprob_back_kernel, LogitRows a, CoefArgs k) {
+  const int64_t r = row_of<NT>(a.batch * a.seq);
+  if (r < 0) return;
+  const int64_t b = r / a.seq, t = r % a.seq;
+  R row;
+  if (a.mask && !a.mask[r]) {
+    row.zero(k.dz, r * a.vocab, a.vocab);
+    return;
+  }
+  float c = k.coef[b * k.batch_stride + t * k.row_stride];
+  if (k.scale) c *= *k.scale;
   const int64_t y = a.targets[r];
   if (y < 0 || y >= a.vocab) c = __builtin_nanf("");
-  row_grad<DT>(a, b * a.batch_stride + t * a.row_stride, y, stats[r].x, stats[r].y, c, dz, r * a.vocab);
+  row.load(a.z, b * a.batch_stride + t * a.row_stride, a.vocab);
+  row.grad(k.dz, r * a.vocab, y < a.vocab ? y : -1, {k.stats[r].x, k.stats[r].y}, c);
 }
 
 // ---------------------------------------------------------- policy loss ---
@@ -132,35 +337,40 @@ __global__ void __launch_bounds__(1024) policy_weight_kernel(PolicyArgs a) {
   }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kRowThreads) policy_kernel(PolicyArgs a) {
-  __shared__ float scratch[16];
+ROW_KERNEL(R, NT, policy_kernel, PolicyArgs a) {
+  __shared__ float2 scratch[16];
   const LogitRows &q = a.rows;
-  const int64_t r = blockIdx.x, b = r / q.seq, t = r % q.seq;
+  const int64_t r = row_of<NT>(q.batch * q.seq);
+  if (r < 0) return;
+  const int lane = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
+  const int64_t b = r / q.seq, t = r % q.seq;
+  R row;
   if (q.mask && !q.mask[r]) {
-    if (threadIdx.x == 0) a.logprobs[r] = a.terms[r] = 0.f;
-    if (a.dz) row_zero<DT>(a.dz, r * q.vocab, q.vocab);
+    if (lane == 0) a.logprobs[r] = a.terms[r] = 0.f;
+    if (a.dz) row.zero(a.dz, r * q.vocab, q.vocab);
     return;
   }
   const int64_t at = b * q.batch_stride + t * q.row_stride, y = q.targets[r];
-  const RowLp o = row_lp<DT>(q, at, y, scratch);
+  row.load(q.z, at, q.vocab);
+  const RowStat o = row.stat(scratch);
+  const float lp = target_lp<DT>(q, at, y, o);
   const float w = a.weights[b], adv = a.adv[b * a.adv_batch + t * a.adv_seq];
-  const float ratio = a.old_lp ? expf(o.lp - a.old_lp[r]) : 1.f;
+  const float ratio = a.old_lp ? expf(lp - a.old_lp[r]) : 1.f;
   // (comparisons that keep a NaN, which fminf and fmaxf would drop)
   const float clipped = ratio < a.low ? a.low : ratio > a.high ? a.high : ratio;
   float term = -(clipped * adv < ratio * adv ? clipped * adv : ratio * adv);
   const bool moves = adv > 0.f ? ratio <= a.high : ratio >= a.low;
   float c = moves ? -ratio * adv : 0.f;
   if (a.ref_lp) {
-    const float gap = a.ref_lp[r] - o.lp, em1 = expm1f(gap);
+    const float gap = a.ref_lp[r] - lp, em1 = expm1f(gap);
     term += a.kl * (em1 - gap);
     c -= a.kl * em1;
   }
-  if (threadIdx.x == 0) {
-    a.logprobs[r] = o.lp;
+  if (lane == 0) {
+    a.logprobs[r] = lp;
     a.terms[r] = w * term;
   }
-  if (a.dz) row_grad<DT>(q, at, y, o.top, o.sum, w * c, a.dz, r * q.vocab);
+  if (a.dz) row.grad(a.dz, r * q.vocab, y < q.vocab ? y : -1, o, w * c);
 }
 
 __global__ void __launch_bounds__(1024) sum_kernel(const float *x, int64_t n, float *out) {
@@ -234,15 +444,36 @@ static int logits_check(const char *what, const void *z, int dtype, int64_t batc
   return SMX_OK;
 }
 
-#define LOGITS_BY_DTYPE(dtype, LAUNCH) \
-  do {                                 \
-    if ((dtype) == SMX_F32) {          \
-      LAUNCH(SMX_F32);                 \
-    } else if ((dtype) == SMX_BF16) {  \
-      LAUNCH(SMX_BF16);                \
-    } else {                           \
-      LAUNCH(SMX_F16);                 \
-    }                                  \
+// Threads and chunks by the row's length in 16-byte chunks: a wave a row (four
+// rows a block) up to 4 KB, so that a short row waits for no other wave; then
+// 256, 512 and 1024 threads with up to 16 chunks each, the fewest that hold
+// the row, so that several rows share a CU; past 256 KB the row is read twice.
+#define LOGITS_BY_ROW(DT, vocab, rows, NAME, ...)                                                                   \
+  do {                                                                                                              \
+    const int64_t chunks_ = ceil_div(vocab, Logit<DT>::kPer);                                                       \
+    const unsigned rows_ = static_cast<unsigned>(rows);                                                             \
+    if (chunks_ <= 256) {                                                                                           \
+      hipLaunchKernelGGL((NAME<DT, Row<DT, 64, 4>, 64>), dim3((rows_ + 3) / 4), dim3(256), 0, st, __VA_ARGS__);      \
+    } else if (chunks_ <= 4096) {                                                                                   \
+      hipLaunchKernelGGL((NAME<DT, Row<DT, 256, 16>, 256>), dim3(rows_), dim3(256), 0, st, __VA_ARGS__);            \
+    } else if (chunks_ <= 8192) {                                                                                   \
+      hipLaunchKernelGGL((NAME<DT, Row<DT, 512, 16>, 512>), dim3(rows_), dim3(512), 0, st, __VA_ARGS__);            \
+    } else if (chunks_ <= 16384) {                                                                                  \
+      hipLaunchKernelGGL((NAME<DT, Row<DT, 1024, 16>, 1024>), dim3(rows_), dim3(1024), 0, st, __VA_ARGS__);         \
+    } else {                                                                                                        \
+      hipLaunchKernelGGL((NAME<DT, LongRow<DT>, 1024>), dim3(rows_), dim3(1024), 0, st, __VA_ARGS__);               \
+    }                                                                                                               \
+  } while (0)
+
+#define LOGITS_LAUNCH(dtype, vocab, rows, NAME, ...)                \
+  do {                                                              \
+    if ((dtype) == SMX_F32) {                                       \
+      LOGITS_BY_ROW(SMX_F32, vocab, rows, NAME, __VA_ARGS__);       \
+    } else if ((dtype) == SMX_BF16) {                               \
+      LOGITS_BY_ROW(SMX_BF16, vocab, rows, NAME, __VA_ARGS__);      \
+    } else {                                                        \
+      LOGITS_BY_ROW(SMX_F16, vocab, rows, NAME, __VA_ARGS__);       \
+    }                                                               \
   } while (0)
 
 }  // namespace smx
@@ -256,12 +487,8 @@ extern "C" int smx_token_logprobs(const void *logits, int dtype, int64_t batch, 
   if (rc != SMX_OK || batch * seq == 0) return rc;
   SMX_REQUIRE(logprobs, SMX_EINVAL, "token_logprobs: null output");
   const LogitRows a{logits, targets, mask, batch, seq, vocab, batch_stride, row_stride};
-  const dim3 grid(static_cast<unsigned>(batch * seq));
-#define LAUNCH(DT) \
-  hipLaunchKernelGGL((logprob_kernel<DT>), grid, dim3(kRowThreads), 0, static_cast<hipStream_t>(stream), a, logprobs, \
-                     reinterpret_cast<float2 *>(stats))
-  LOGITS_BY_DTYPE(dtype, LAUNCH);
-#undef LAUNCH
+  const auto st = static_cast<hipStream_t>(stream);
+  LOGITS_LAUNCH(dtype, vocab, batch * seq, logprob_kernel, a, logprobs, reinterpret_cast<float2 *>(stats));
   return check_launch("token_logprobs");
 }
 
@@ -274,12 +501,9 @@ extern "C" int smx_token_logprobs_backward(const void *logits, int dtype, int64_
   if (rc != SMX_OK || batch * seq == 0) return rc;
   SMX_REQUIRE(stats && coef && dlogits, SMX_EINVAL, "token_logprobs_backward: null pointer");
   const LogitRows a{logits, targets, mask, batch, seq, vocab, batch_stride, row_stride};
-  const dim3 grid(static_cast<unsigned>(batch * seq));
-#define LAUNCH(DT)                                                                                                    \
-  hipLaunchKernelGGL((logprob_back_kernel<DT>), grid, dim3(kRowThreads), 0, static_cast<hipStream_t>(stream), a,    \
-                     reinterpret_cast<const float2 *>(stats), coef, coef_batch_stride, coef_row_stride, scale, dlogits)
-  LOGITS_BY_DTYPE(dtype, LAUNCH);
-#undef LAUNCH
+  const CoefArgs k{reinterpret_cast<const float2 *>(stats), coef, scale, coef_batch_stride, coef_row_stride, dlogits};
+  const auto st = static_cast<hipStream_t>(stream);
+  LOGITS_LAUNCH(dtype, vocab, batch * seq, logprob_back_kernel, a, k);
   return check_launch("token_logprobs_backward");
 }
 
@@ -315,10 +539,7 @@ extern "C" int smx_policy_loss(const void *logits, int dtype, int64_t batch, int
     a.per_sequence = reduction == SMX_MEAN_SEQUENCE;
     a.logprobs = logprobs, a.weights = static_cast<float *>(workspace), a.terms = a.weights + batch, a.dz = dlogits;
     hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a);
-    const dim3 grid(static_cast<unsigned>(rows));
-#define LAUNCH(DT) hipLaunchKernelGGL((policy_kernel<DT>), grid, dim3(kRowThreads), 0, st, a)
-    LOGITS_BY_DTYPE(dtype, LAUNCH);
-#undef LAUNCH
+    LOGITS_LAUNCH(dtype, vocab, rows, policy_kernel, a);
   }
   hipLaunchKernelGGL(sum_kernel, dim3(1), dim3(1024), 0, st, static_cast<const float *>(a.terms), rows, loss);
   return check_launch("policy_loss");
@@ -342,8 +563,13 @@ extern "C" int smx_scale(void *x, int dtype, int64_t n, const float *scale, void
   if (n == 0) return SMX_OK;
   SMX_REQUIRE(x && scale, SMX_EINVAL, "scale: null pointer");
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(4096, ceil_div(n, 256))));
-#define LAUNCH(DT) hipLaunchKernelGGL((scale_kernel<DT>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), x, n, scale)
-  LOGITS_BY_DTYPE(dtype, LAUNCH);
-#undef LAUNCH
+  const auto st = static_cast<hipStream_t>(stream);
+  if (dtype == SMX_F32) {
+    hipLaunchKernelGGL((scale_kernel<SMX_F32>), grid, dim3(256), 0, st, x, n, scale);
+  } else if (dtype == SMX_BF16) {
+    hipLaunchKernelGGL((scale_kernel<SMX_BF16>), grid, dim3(256), 0, st, x, n, scale);
+  } else {
+    hipLaunchKernelGGL((scale_kernel<SMX_F16>), grid, dim3(256), 0, st, x, n, scale);
+  }
   return check_launch("scale");
 }
