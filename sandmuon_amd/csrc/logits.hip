@@ -22,11 +22,22 @@ struct LogitRows {
 // ------------------------------------------------------------- one row ---
 // A row is held in registers from its one read to its gradient's one write:
 // NT threads with up to NCH 16-byte chunks each, all of whose loads are in
-// flight at once.  Chunks begin at the row's first element, at the elements'
-// own alignment (an odd vocabulary moves every row's start), so the sums do
-// not depend on where a row lies; the elements behind the last whole chunk
-// are one of each of the first threads.
+// flight at once.  An odd vocabulary moves every row's start: the chunks of a
+// long row begin at its first 16-byte boundary, since loads that straddle
+// boundaries cost a tenth of the time (8 x 1024 x 50257 bf16: 333 us, 296 us
+// with aligned ones), and which elements a thread sums then depends on where
+// the row lies.  A row of one wave (NT = 64) is bound by latency, not by that,
+// and takes its chunks from its first element, so that its sums are the same
+// wherever it lies.  The elements before the first chunk and behind the last
+// (at most 7 and 7 of 16 bits) are one of each of the first 16 threads.
 typedef uint32_t v4u_any __attribute__((ext_vector_type(4), aligned(2)));
+
+// Elements of a row before its first chunk.
+template <int NT>
+__device__ __forceinline__ int row_head(const char *row, int bytes, int vocab) {
+  if constexpr (NT == 64) return 0;
+  return min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / bytes, vocab);
+}
 
 template <int DT>
 struct Logit {
@@ -91,26 +102,32 @@ template <int DT, int NT, int NCH>
 struct Row {
   using L = Logit<DT>;
   uint4 c[NCH];
-  float edge;   // this thread's element behind the whole chunks
-  int edge_at;  // its place, or -1
-  int chunks;   // whole chunks
+  float edge;       // this thread's element outside the whole chunks
+  int edge_at;      // its place, or -1
+  int chunks, head;  // whole chunks, elements before them
   int tid;
   const char *src;
 
+  template <bool AGAIN>
   __device__ __forceinline__ void load(const void *z, int64_t at, int64_t vocab) {
     const char *row = src = static_cast<const char *>(z) + at * L::kBytes;
     tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
     const int v = static_cast<int>(vocab);
-    chunks = v / L::kPer;
+    head = row_head<NT>(row, L::kBytes, v);
+    chunks = (v - head) / L::kPer;
+    const char *p = row + head * L::kBytes;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       c[i] = make_uint4(L::kNone, L::kNone, L::kNone, L::kNone);
       if (i * NT < chunks && tid + i * NT < chunks) {
-        const v4u_any w = __builtin_nontemporal_load(reinterpret_cast<const v4u_any *>(row) + tid + i * NT);
+        // (AGAIN: the row is read once more later, and may stay in a cache)
+        const auto *at_i = reinterpret_cast<const v4u_any *>(p) + tid + i * NT;
+        const v4u_any w = AGAIN ? *at_i : __builtin_nontemporal_load(at_i);
         c[i] = make_uint4(w.x, w.y, w.z, w.w);
       }
     }
-    edge_at = tid < v - chunks * L::kPer ? chunks * L::kPer + tid : -1;
+    const int tail = head + chunks * L::kPer;
+    edge_at = tid < 8 ? (tid < head ? tid : -1) : tid < 16 && tail + tid - 8 < v ? tail + tid - 8 : -1;
     edge = edge_at >= 0 ? load_elem<DT>(row, edge_at) : -INFINITY;
   }
 
@@ -168,8 +185,8 @@ struct Row {
     }
     if (edge_at >= 0) store_any(row, DT, edge_at, round_to(DT, exp_of<DT>(edge - r.top) * scale));
     // the target's element again, by the thread that wrote it
-    const int t = static_cast<int>(y);
-    const bool mine = t >= chunks * L::kPer ? t == edge_at : tid == t / L::kPer % NT;
+    const int t = static_cast<int>(y) - head;
+    const bool mine = t < 0 || t >= chunks * L::kPer ? static_cast<int>(y) == edge_at : tid == t / L::kPer % NT;
     if (y >= 0 && mine)
       store_any(row, DT, y, round_to(DT, fmaf(exp_of<DT>(load_elem<DT>(src, y) - r.top), scale, coef)));
   }
@@ -178,14 +195,19 @@ struct Row {
     char *row = static_cast<char *>(out) + at * L::kBytes;
     tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
     const int v = static_cast<int>(vocab);
-    chunks = v / L::kPer;
+    head = row_head<NT>(row, L::kBytes, v);
+    chunks = (v - head) / L::kPer;
     for (int i = 0; i * NT < chunks; ++i)
       if (tid + i * NT < chunks) put(row, i, make_uint4(0, 0, 0, 0));
-    if (tid < v - chunks * L::kPer) store_any(row, DT, chunks * L::kPer + tid, 0.f);
+    const int tail = head + chunks * L::kPer;
+    if (tid < head) store_any(row, DT, tid, 0.f);
+    if (tid < v - tail) store_any(row, DT, tail + tid, 0.f);
   }
 
+  // Chunk i of this thread, at the alignment of the output's row, which need
+  // not be the input's.
   __device__ __forceinline__ void put(char *row, int i, const uint4 &w) const {
-    __builtin_nontemporal_store(v4u_any{w.x, w.y, w.z, w.w}, reinterpret_cast<v4u_any *>(row) + tid + i * NT);
+    __builtin_nontemporal_store(v4u_any{w.x, w.y, w.z, w.w}, reinterpret_cast<v4u_any *>(row + head * L::kBytes) + tid + i * NT);
   }
 };
 
@@ -196,6 +218,7 @@ struct LongRow {
   static constexpr int NT = 1024;
   const void *z;
   int64_t at, vocab;
+  template <bool AGAIN>
   __device__ __forceinline__ void load(const void *p, int64_t i, int64_t v) { z = p, at = i, vocab = v; }
   __device__ __forceinline__ RowStat stat(float2 *scratch) const {
     float m = -INFINITY, s = 0.f;
@@ -267,7 +290,11 @@ ROW_KERNEL(R, NT, logprob_kernel, LogitRows a, float *logprobs, float2 *stats) {
   }
   const int64_t at = r / a.seq * a.batch_stride + r % a.seq * a.row_stride, y = a.targets[r];
   R row;
-  row.load(a.z, at, a.vocab);
+  if (stats) {
+    row.template load<true>(a.z, at, a.vocab);
+  } else {
+    row.template load<false>(a.z, at, a.vocab);
+  }
   const RowStat o = row.stat(scratch);
   const float lp = target_lp<DT>(a, at, y, o);
   if (lane == 0) {
@@ -284,8 +311,11 @@ struct CoefArgs {
 };
 
 ROW_KERNEL(R, NT, logprob_back_kernel, LogitRows a, CoefArgs k) {
-  const int64_t r = row_of<NT>(a.batch * a.seq);
+  int64_t r = row_of<NT>(a.batch * a.seq);
   if (r < 0) return;
+  // The rows that the forward read last first: what the last cache still holds
+  // of them is read from it.
+  r = a.batch * a.seq - 1 - r;
   const int64_t b = r / a.seq, t = r % a.seq;
   R row;
   if (a.mask && !a.mask[r]) {
@@ -296,7 +326,7 @@ ROW_KERNEL(R, NT, logprob_back_kernel, LogitRows a, CoefArgs k) {
   if (k.scale) c *= *k.scale;
   const int64_t y = a.targets[r];
   if (y < 0 || y >= a.vocab) c = __builtin_nanf("");
-  row.load(a.z, b * a.batch_stride + t * a.row_stride, a.vocab);
+  row.template load<false>(a.z, b * a.batch_stride + t * a.row_stride, a.vocab);
   row.grad(k.dz, r * a.vocab, y < a.vocab ? y : -1, {k.stats[r].x, k.stats[r].y}, c);
 }
 
@@ -351,7 +381,7 @@ ROW_KERNEL(R, NT, policy_kernel, PolicyArgs a) {
     return;
   }
   const int64_t at = b * q.batch_stride + t * q.row_stride, y = q.targets[r];
-  row.load(q.z, at, q.vocab);
+  row.template load<false>(q.z, at, q.vocab);
   const RowStat o = row.stat(scratch);
   const float lp = target_lp<DT>(q, at, y, o);
   const float w = a.weights[b], adv = a.adv[b * a.adv_batch + t * a.adv_seq];
@@ -445,15 +475,15 @@ static int logits_check(const char *what, const void *z, int dtype, int64_t batc
 }
 
 // Threads and chunks by the row's length in 16-byte chunks: a wave a row (four
-// rows a block) up to 4 KB, so that a short row waits for no other wave; then
+// rows a block) up to 8 KB, so that a short row waits for no other wave; then
 // 256, 512 and 1024 threads with up to 16 chunks each, the fewest that hold
 // the row, so that several rows share a CU; past 256 KB the row is read twice.
 #define LOGITS_BY_ROW(DT, vocab, rows, NAME, ...)                                                                   \
   do {                                                                                                              \
     const int64_t chunks_ = ceil_div(vocab, Logit<DT>::kPer);                                                       \
     const unsigned rows_ = static_cast<unsigned>(rows);                                                             \
-    if (chunks_ <= 256) {                                                                                           \
-      hipLaunchKernelGGL((NAME<DT, Row<DT, 64, 4>, 64>), dim3((rows_ + 3) / 4), dim3(256), 0, st, __VA_ARGS__);      \
+    if (chunks_ <= 512) {                                                                                           \
+      hipLaunchKernelGGL((NAME<DT, Row<DT, 64, 8>, 64>), dim3((rows_ + 3) / 4), dim3(256), 0, st, __VA_ARGS__);      \
     } else if (chunks_ <= 4096) {                                                                                   \
       hipLaunchKernelGGL((NAME<DT, Row<DT, 256, 16>, 256>), dim3(rows_), dim3(256), 0, st, __VA_ARGS__);            \
     } else if (chunks_ <= 8192) {                                                                                   \
