@@ -15,6 +15,39 @@ namespace smx {
 
 constexpr int kActRows = 4;
 
+// Two values rounded to nearest even in a 16-bit type.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  uint32_t w;
+  if constexpr (DT == SMX_BF16) {
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    const v2bf h = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+    __builtin_memcpy(&w, &h, 4);
+  } else {
+    const _Float16 h[2] = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+    __builtin_memcpy(&w, h, 4);
+  }
+  return w;
+}
+
+// Eight values as their type holds them.
+template <int DT>
+__device__ __forceinline__ void round8(float *v) {
+  if constexpr (DT != SMX_F32) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t w = pack2<DT>(v[2 * k], v[2 * k + 1]);
+      if constexpr (DT == SMX_BF16) {
+        v[2 * k] = __uint_as_float(w << 16);
+        v[2 * k + 1] = __uint_as_float(w & 0xffff0000u);
+      } else {
+        v[2 * k] = f16_bits_to_f32(static_cast<uint16_t>(w));
+        v[2 * k + 1] = f16_bits_to_f32(static_cast<uint16_t>(w >> 16));
+      }
+    }
+  }
+}
+
 template <int DT, bool VEC>
 struct Elems8 {
   // Elements [i, i + n) of p, n <= 8; the rest are zero.
@@ -53,20 +86,13 @@ struct Elems8 {
       } else {
         uint32_t w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if constexpr (DT == SMX_BF16) {
-            w[k] = f32_to_bf16_bits(v[2 * k]) | (static_cast<uint32_t>(f32_to_bf16_bits(v[2 * k + 1])) << 16);
-          } else {
-            const _Float16 h[2] = {static_cast<_Float16>(v[2 * k]), static_cast<_Float16>(v[2 * k + 1])};
-            __builtin_memcpy(&w[k], h, 4);
-          }
-        }
+        for (int k = 0; k < 4; ++k) w[k] = pack2<DT>(v[2 * k], v[2 * k + 1]);
         *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (k < n) store_any(p, DT, i + k, v[k]);
+        if (k < n) store_any(p, DT, i + k, round_to(DT, v[k]));
     }
   }
 };
@@ -111,8 +137,49 @@ struct Act8Args {
   int64_t rows, cols, pitch, x_stride, y_stride, dy_stride;
 };
 
-// FP32 GELU in torch's order of operations: x * 0.5 * (1 + erf(x / sqrt 2)).
-__device__ __forceinline__ float act8_phi(float x) { return 0.5f * (1.f + erff(x * 0.70710678118654752f)); }
+// FP32 in torch's order of operations: x * 0.5 * (1 + erf(x / sqrt 2)).
+__device__ __forceinline__ float phi_f32(float x) { return 0.5f * (1.f + erff(x * 0.70710678118654752f)); }
+
+// For 16-bit types, whose half place is 2^-12 at the least: the normal tail
+// Q(x) = (1 - erf(x / sqrt 2)) / 2 of x >= 0 as exp(-x^2 / 2) times a polynomial
+// of degree 8 in t = 1 / (1 + 0.3175 x), a least-squares fit of this file's own,
+// reweighted towards the largest error, of exp(x^2 / 2) Q(x) on [0, 40] (Q
+// underflows beyond 14): 3.5e-7 off, and 3e-7 as evaluated.  (Degree 6, 1.1e-5
+// off, is not enough for the slope near its zero.)  About half of erff's vector
+// instructions, which would bound the kernel, not HBM.
+struct NormalTail {
+  float e, q;  // exp(-x^2 / 2), Q(x)
+};
+__device__ __forceinline__ NormalTail normal_tail(float x) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3175f, x, 1.f));
+  float g = fmaf(t, 0.03485208749771118f, -0.1270199567079544f);
+  g = fmaf(t, g, 0.11735344678163528f);
+  g = fmaf(t, g, 0.009273595176637173f);
+  g = fmaf(t, g, 0.09985337406396866f);
+  g = fmaf(t, g, 0.11224232614040375f);
+  g = fmaf(t, g, 0.12678450345993042f);
+  g = fmaf(t, g, 0.1266608089208603f);
+  const float e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);
+  return {e, e * (t * g)};
+}
+
+// GELU(h) = max(h, 0) - |h| Q(|h|), keeping infinities and NaN as the formula
+// h Phi(h) does (-inf gives NaN).
+template <int DT>
+__device__ __forceinline__ float gelu_of(float h) {
+  if constexpr (DT == SMX_F32) return h * phi_f32(h);
+  const float x = fminf(fabsf(h), 40.f);
+  return fmaf(-x, normal_tail(x).q, fmaf(0.5f, fabsf(h), 0.5f * h));
+}
+
+// GELU'(h) = Phi(h) + h phi(h).
+template <int DT>
+__device__ __forceinline__ float gelu_slope(float h) {
+  constexpr float kPhi0 = 0.3989422804014327f;
+  if constexpr (DT == SMX_F32) return phi_f32(h) + h * (expf(-0.5f * h * h) * kPhi0);
+  const NormalTail n = normal_tail(fminf(fabsf(h), 40.f));
+  return fmaf(h, n.e * kPhi0, 0.5f + copysignf(0.5f - n.q, h));
+}
 
 enum Act8Op : int { kActEncode = 0, kActGelu = 1, kActDecode = 2, kActGeluBack = 3 };
 
@@ -153,7 +220,8 @@ __global__ void __launch_bounds__(256) act8_kernel(Act8Args a) {
       if constexpr (OP == kActGelu) {
         // (the output is kept as it is stored: rounded to its type first)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[u][k] = round_to(DT, v[u][k] * act8_phi(v[u][k]));
+        for (int k = 0; k < 8; ++k) v[u][k] = gelu_of<DT>(v[u][k]);
+        round8<DT>(v[u]);
         if (n > 0) E::store(a.y, r * a.y_stride + 8 * chunk, n, v[u]);
         if (a.y8.codes) act8_put<FMT>(v[u], a.y8, r, a.pitch, chunk);
       }
@@ -165,11 +233,8 @@ __global__ void __launch_bounds__(256) act8_kernel(Act8Args a) {
         act8_unpack4<FMT>(codes[u].y, scale, h + 4);
         if constexpr (OP == kActGeluBack) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            h[k] = v[u][k] * (act8_phi(h[k]) + h[k] * (expf(-0.5f * h[k] * h[k]) * 0.3989422804014327f));
+          for (int k = 0; k < 8; ++k) h[k] = v[u][k] * gelu_slope<DT>(h[k]);
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) h[k] = round_to(DT, h[k]);
         E::store(a.y, r * a.y_stride + 8 * chunk, n, h);
       }
     }
