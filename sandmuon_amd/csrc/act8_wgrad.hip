@@ -29,16 +29,22 @@ struct WgradArgs {
   const void *delta;  // [rows, n] of its dtype
   const uint8_t *codes, *scales;
   void *dw;            // [n, k], or the splits' partial tiles [splits, n, k] in FP32
-  void *db;            // [n], or [splits, n] in FP32, or null
+  float *db;           // partial column sums [splits, tiles_k, n], or null
   int64_t rows, n, k, pitch, delta_stride;
   int64_t split_rows;  // rows of a split, a multiple of the step
   int32_t tiles_k, tiles, splits, out;
 };
 
-constexpr int kWgThreads = 256;
 constexpr int parts_of(int dt) { return dt == SMX_BF16 ? 1 : dt == SMX_F16 ? 2 : 3; }
-// Rows of a step: its MFMAs (one product per part) cover the loads of the next.
-constexpr int wgrad_step(int dt, int tile) { return tile == 256 && dt != SMX_BF16 ? 32 : 64; }
+
+// Tiles: rows and columns, the waves that share them, and the rows of a step.
+template <int TN, int TK, int WN, int WK, int STEP, int STEP_PARTS, int WPS>
+struct WgradTile {
+  static constexpr int kTileN = TN, kTileK = TK, kWavesN = WN, kWavesK = WK, kThreads = 64 * WN * WK, kWavesPerSimd = WPS;
+  static constexpr int step(int dt) { return dt == SMX_BF16 ? STEP : STEP_PARTS; }
+};
+using WgradWide = WgradTile<256, 256, 2, 4, 64, 32, 2>;
+using WgradSmall = WgradTile<128, 128, 2, 2, 64, 32, 2>;
 
 // 16 codes and their scale to 16 BF16 values (two uint4).
 template <int FMT>
@@ -128,12 +134,14 @@ __device__ __forceinline__ int lds_at(int row, int block) {
   return row * 2 * T + ((block ^ ((row & 3) << 1)) << 5);
 }
 
-template <int DT, int FMT, int T>
-__global__ void __launch_bounds__(kWgThreads) wgrad_kernel(WgradArgs a) {
-  constexpr int P = parts_of(DT), kStep = wgrad_step(DT, T);
-  constexpr int kPlane = kStep * T * 2, kBuffer = (P + 1) * kPlane;
-  constexpr int kDeltaLoads = kStep * T / 8 / kWgThreads, kCodeLoads = kStep * T / 16 / kWgThreads;
-  constexpr int W = T / 2, F = W / 32;  // a wave's tile of W x W, in F x F MFMA tiles
+template <int DT, int FMT, class C>
+__global__ void __launch_bounds__(C::kThreads, C::kWavesPerSimd) wgrad_kernel(WgradArgs a) {
+  constexpr int P = parts_of(DT), kStep = C::step(DT), TN = C::kTileN, TK = C::kTileK;
+  constexpr int kPlane = kStep * TN * 2, kBuffer = P * kPlane + kStep * TK * 2;
+  constexpr int kDeltaRows = C::kThreads / (TN / 8), kCodeRows = C::kThreads / (TK / 16);  // rows of one pass of loads
+  constexpr int kDeltaLoads = kStep / kDeltaRows, kCodeLoads = kStep / kCodeRows;
+  static_assert(kDeltaLoads * kDeltaRows == kStep && kCodeLoads * kCodeRows == kStep, "whole passes");
+  constexpr int FN = TN / C::kWavesN / 32, FK = TK / C::kWavesK / 32;  // a wave's MFMA tiles
   __shared__ __attribute__((aligned(128))) char lds[2 * kBuffer];
 
   // Blocks of one split run on one XCD as far as they can, since they share its rows.
@@ -142,18 +150,19 @@ __global__ void __launch_bounds__(kWgThreads) wgrad_kernel(WgradArgs a) {
   const int64_t id = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
   if ((blockIdx.x >> 3) >= share || id >= blocks) return;
   const int split = static_cast<int>(id / a.tiles), tile = static_cast<int>(id % a.tiles);
-  const int64_t n0 = static_cast<int64_t>(tile / a.tiles_k) * T, k0 = static_cast<int64_t>(tile % a.tiles_k) * T;
+  const int tile_k = tile % a.tiles_k;
+  const int64_t n0 = static_cast<int64_t>(tile / a.tiles_k) * TN, k0 = static_cast<int64_t>(tile_k) * TK;
   const int64_t m_begin = split * a.split_rows, m_end = min(a.rows, m_begin + a.split_rows);
   const int steps = static_cast<int>((m_end - m_begin + kStep - 1) / kStep);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wn = (wave >> 1) * W, wk = (wave & 1) * W;
+  const int wn = wave / C::kWavesK * (32 * FN), wk = wave % C::kWavesK * (32 * FK);
 
   // Staging: a thread loads 8 cotangents (16 codes) of the same columns in
   // every row of its own.  Columns past the end repeat others in bounds: what
   // they add to is not stored.
-  const int d_row = tid / (T / 8), d_col = tid % (T / 8);
-  const int c_row = tid / (T / 16), c_col = tid % (T / 16);
+  const int d_row = tid / (TN / 8), d_col = tid % (TN / 8);
+  const int c_row = tid / (TK / 16), c_col = tid % (TK / 16);
   const int64_t nc = min(n0 + 8 * d_col, (a.n - 1) & ~int64_t{7});
   const int nc_count = static_cast<int>(min<int64_t>(8, a.n - nc));
   const int64_t kc = min(k0 + 16 * c_col, a.pitch - 16);
@@ -163,7 +172,6 @@ __global__ void __launch_bounds__(kWgThreads) wgrad_kernel(WgradArgs a) {
   uint4 c[kCodeLoads];
   int s[kCodeLoads];
   float sum[8] = {};
-  const bool bias = a.db && k0 == 0;
 
   const auto load = [&](int step) __attribute__((always_inline)) {
     const int64_t m0 = m_begin + static_cast<int64_t>(step) * kStep;
@@ -173,22 +181,22 @@ __global__ void __launch_bounds__(kWgThreads) wgrad_kernel(WgradArgs a) {
     if (m0 + kStep < a.rows && m0 + kStep <= m_end && a.n >= 8 && a.k > 0) {
 #pragma unroll
       for (int i = 0; i < kDeltaLoads; ++i)
-        d[i].load(a.delta, (m0 + d_row + i * (kStep / kDeltaLoads)) * a.delta_stride + nc);
+        d[i].load(a.delta, (m0 + d_row + i * kDeltaRows) * a.delta_stride + nc);
 #pragma unroll
       for (int i = 0; i < kCodeLoads; ++i) {
-        const int64_t m = m0 + c_row + i * (kStep / kCodeLoads);
+        const int64_t m = m0 + c_row + i * kCodeRows;
         c[i] = *reinterpret_cast<const uint4 *>(a.codes + m * a.pitch + kc);
         s[i] = a.scales[m * scale_pitch + (kc >> 5)];
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kDeltaLoads; ++i) {
-        const int64_t m = m0 + d_row + i * (kStep / kDeltaLoads);
+        const int64_t m = m0 + d_row + i * kDeltaRows;
         d[i].load_some(a.delta, m * a.delta_stride + nc, m < m_end ? nc_count : 0);
       }
 #pragma unroll
       for (int i = 0; i < kCodeLoads; ++i) {
-        const int64_t m = m0 + c_row + i * (kStep / kCodeLoads);
+        const int64_t m = m0 + c_row + i * kCodeRows;
         c[i] = make_uint4(0, 0, 0, 0);
         s[i] = 1;
         if (m < m_end && a.k > 0) {
@@ -198,77 +206,84 @@ __global__ void __launch_bounds__(kWgThreads) wgrad_kernel(WgradArgs a) {
       }
     }
   };
-  const auto stage = [&](int buffer) __attribute__((always_inline)) {
-    char *at = lds + buffer * kBuffer;
+  const auto stage_delta = [&](char *at, int i) __attribute__((always_inline)) {
+    const int row = d_row + i * kDeltaRows;
+    uint4 o[P];
+    d[i].parts(o);
 #pragma unroll
-    for (int i = 0; i < kDeltaLoads; ++i) {
-      const int row = d_row + i * (kStep / kDeltaLoads);
-      uint4 o[P];
-      d[i].parts(o);
+    for (int p = 0; p < P; ++p)
+      *reinterpret_cast<uint4 *>(at + p * kPlane + lds_at<TN>(row, d_col >> 1) + (d_col & 1) * 16) = o[p];
+  };
+  const auto stage_codes = [&](char *at, int i) __attribute__((always_inline)) {
+    const int row = c_row + i * kCodeRows;
+    uint4 o[2];
+    act8_to_bf16<FMT>(c[i], s[i], o);
+    uint4 *to = reinterpret_cast<uint4 *>(at + P * kPlane + lds_at<TK>(row, c_col));
+    to[0] = o[0], to[1] = o[1];
+  };
+  // The column sums for db, of the steps whose turn it is: each of the row of
+  // tiles that share these cotangents takes its share.
+  const auto add_bias = [&](int step) __attribute__((always_inline)) {
+    if (!a.db || step % a.tiles_k != tile_k) return;
 #pragma unroll
-      for (int p = 0; p < P; ++p)
-        *reinterpret_cast<uint4 *>(at + p * kPlane + lds_at<T>(row, d_col >> 1) + (d_col & 1) * 16) = o[p];
-    }
-    if (bias) {
+    for (int i = 0; i < kDeltaLoads; ++i)
 #pragma unroll
-      for (int i = 0; i < kDeltaLoads; ++i)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sum[k] += d[i].value(k);
-    }
-#pragma unroll
-    for (int i = 0; i < kCodeLoads; ++i) {
-      const int row = c_row + i * (kStep / kCodeLoads);
-      uint4 o[2];
-      act8_to_bf16<FMT>(c[i], s[i], o);
-      uint4 *to = reinterpret_cast<uint4 *>(at + P * kPlane + lds_at<T>(row, c_col));
-      to[0] = o[0], to[1] = o[1];
-    }
+      for (int k = 0; k < 8; ++k) sum[k] += d[i].value(k);
   };
 
   // Transposing reads: lane i of a group of 16 names four columns of row
   // i / 4 and receives column i of four rows; groups 0 and 1 hold columns 0-15
   // and 16-31 of rows 0-7 of a 16-row operand, groups 2 and 3 rows 8-15.
   const int g = lane >> 4, i16 = lane & 15, r4 = i16 >> 2;
-  int a_at[F], b_at[F];
+  const int tr_row = 8 * (g >> 1) + r4;
+  int a_at[FN], b_at[FK];
 #pragma unroll
-  for (int f = 0; f < F; ++f) {
-    const int row = 8 * (g >> 1) + r4;
-    a_at[f] = lds_at<T>(row, (wn >> 4) + 2 * f + (g & 1)) + (i16 & 3) * 8;
-    b_at[f] = lds_at<T>(row, (wk >> 4) + 2 * f + (g & 1)) + (i16 & 3) * 8;
-  }
-  const auto operand = [&](const char *at) __attribute__((always_inline)) {
+  for (int f = 0; f < FN; ++f) a_at[f] = lds_at<TN>(tr_row, (wn >> 4) + 2 * f + (g & 1)) + (i16 & 3) * 8;
+#pragma unroll
+  for (int f = 0; f < FK; ++f) b_at[f] = P * kPlane + lds_at<TK>(tr_row, (wk >> 4) + 2 * f + (g & 1)) + (i16 & 3) * 8;
+  const auto operand = [&](const char *at, int four_rows) __attribute__((always_inline)) {
     typedef __attribute__((address_space(3))) v4s *lds_ptr;
     const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at));
-    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 4 * 2 * T));
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + four_rows));
     typedef short v8s __attribute__((ext_vector_type(8)));
     const v8s v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(v8bf, v);
   };
 
-  v16f acc[F][F] = {};
+  v16f acc[FN][FK] = {};
+  const auto stage = [&](char *to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kDeltaLoads; ++i) stage_delta(to, i);
+#pragma unroll
+    for (int i = 0; i < kCodeLoads; ++i) stage_codes(to, i);
+  };
   if (steps > 0) {
     load(0);
-    stage(0);
+    add_bias(0);
+    stage(lds);
   }
   __syncthreads();
   for (int t = 0; t < steps; ++t) {
-    if (t + 1 < steps) load(t + 1);
     const char *at = lds + (t & 1) * kBuffer;
+    if (t + 1 < steps) load(t + 1);
 #pragma unroll
     for (int ms = 0; ms < kStep / 16; ++ms) {
-      v8bf bv[F];
+      v8bf bv[FK];
 #pragma unroll
-      for (int f = 0; f < F; ++f) bv[f] = operand(at + P * kPlane + ms * 16 * 2 * T + b_at[f]);
+      for (int h = 0; h < FK; ++h) bv[h] = operand(at + ms * 16 * 2 * TK + b_at[h], 4 * 2 * TK);
 #pragma unroll
       for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-          const v8bf av = operand(at + p * kPlane + ms * 16 * 2 * T + a_at[f]);
+        for (int f = 0; f < FN; ++f) {
+          const v8bf av = operand(at + p * kPlane + ms * 16 * 2 * TN + a_at[f], 4 * 2 * TN);
 #pragma unroll
-          for (int h = 0; h < F; ++h) acc[f][h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av, bv[h], acc[f][h], 0, 0, 0);
+          for (int h = 0; h < FK; ++h) acc[f][h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av, bv[h], acc[f][h], 0, 0, 0);
         }
     }
-    if (t + 1 < steps) stage((t & 1) ^ 1);
+    if (t + 1 < steps) {
+      add_bias(t + 1);
+      stage(lds + ((t & 1) ^ 1) * kBuffer);
+    }
     __syncthreads();
   }
 
@@ -278,15 +293,15 @@ __global__ void __launch_bounds__(kWgThreads) wgrad_kernel(WgradArgs a) {
     const int64_t nb = n0 + wn, kb = k0 + wk;
     const int ln = 4 * (lane >> 5), lk = lane & 31;
     const uint32_t off = static_cast<uint32_t>(ln) * static_cast<uint32_t>(a.k) + lk;
-    const bool inside = nb + W <= a.n && kb + W <= a.k;
+    const bool inside = nb + 32 * FN <= a.n && kb + 32 * FK <= a.k;
     int64_t at = (a.splits > 1 ? static_cast<int64_t>(split) * a.n * a.k : 0) + nb * a.k + kb;
 #pragma unroll
-    for (int f = 0; f < F; ++f)
+    for (int f = 0; f < FN; ++f)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int row = 32 * f + 8 * (r >> 2) + (r & 3);
 #pragma unroll
-        for (int h = 0; h < F; ++h) {
+        for (int h = 0; h < FK; ++h) {
           float v = acc[f][h][r];
           // (keeps the compiler from moving every sum and address at once)
           asm volatile("" : "+s"(at), "+v"(v));
@@ -303,22 +318,40 @@ __global__ void __launch_bounds__(kWgThreads) wgrad_kernel(WgradArgs a) {
       (static_cast<uint16_t *>(a.dw) + i)[o] = a.out == SMX_BF16 ? f32_to_bf16_bits(v) : __builtin_bit_cast(uint16_t, half);
     });
   }
-  if (bias) {
-    float *red = reinterpret_cast<float *>(lds);  // [rows of threads][T]
+  if (a.db) {
+    float *red = reinterpret_cast<float *>(lds);  // [rows of threads][TN]
 #pragma unroll
-    for (int k = 0; k < 8; ++k) red[d_row * T + 8 * d_col + k] = sum[k];
+    for (int k = 0; k < 8; ++k) red[d_row * TN + 8 * d_col + k] = sum[k];
     __syncthreads();
-    if (tid < T && n0 + tid < a.n) {
+    if (tid < TN && n0 + tid < a.n) {
       float t = 0.f;
-      for (int q = 0; q < kWgThreads / (T / 8); ++q) t += red[q * T + tid];
-      store_any(a.db, a.out, (a.splits > 1 ? split * a.n : 0) + n0 + tid, round_to(a.out, t));
+      for (int q = 0; q < kDeltaRows; ++q) t += red[q * TN + tid];
+      a.db[(static_cast<int64_t>(split) * a.tiles_k + tile_k) * a.n + n0 + tid] = t;
     }
   }
 }
 
-// The splits' partial sums added in order.
+// The splits' partial sums added in order: dw (count = 0: it is whole), then db
+// of `db_parts` parts: a block per 1024 elements of dw, then one per 16 of db.
 __global__ void __launch_bounds__(256) wgrad_join_kernel(const float *part, int64_t count, int splits, void *out,
-                                                         int out_dtype, const float *part_db, int64_t n, void *db) {
+                                                         int out_dtype, const float *part_db, int64_t n, int db_parts,
+                                                         void *db) {
+  const int64_t dw_blocks = (count + 1023) / 1024;
+  if (static_cast<int64_t>(blockIdx.x) >= dw_blocks) {
+    // 16 columns of db, each from 16 threads
+    __shared__ float red[16][17];
+    const int col = threadIdx.x & 15, q = threadIdx.x >> 4;
+    const int64_t j = (blockIdx.x - dw_blocks) * 16 + col;
+    float t = 0.f;
+    if (j < n)
+      for (int s = q; s < db_parts; s += 16) t += part_db[s * n + j];
+    red[q][col] = t;
+    __syncthreads();
+    if (q > 0 || j >= n) return;
+    for (int s = 1; s < 16; ++s) t += red[s][col];
+    store_any(db, out_dtype, j, round_to(out_dtype, t));
+    return;
+  }
   const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
   if (i0 + 4 <= count && count % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
     float4 t = make_float4(0, 0, 0, 0);
@@ -341,16 +374,11 @@ __global__ void __launch_bounds__(256) wgrad_join_kernel(const float *part, int6
       store_any(out, out_dtype, i, round_to(out_dtype, t));
     }
   }
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (db && j < n) {
-    float t = 0.f;
-    for (int s = 0; s < splits; ++s) t += part_db[s * n + j];
-    store_any(db, out_dtype, j, round_to(out_dtype, t));
-  }
 }
 
 struct WgradPlan {
-  int tile, tiles_n, tiles_k, splits;
+  bool wide;
+  int tiles_n, tiles_k, splits;
   int64_t split_rows;
 };
 
@@ -359,10 +387,12 @@ struct WgradPlan {
 static WgradPlan wgrad_plan(int dtype, int64_t rows, int64_t n, int64_t k) {
   WgradPlan p{};
   constexpr int64_t kCus = 256;
-  p.tile = ceil_div(n, 256) * ceil_div(k, 256) * 4 >= kCus ? 256 : 128;
-  p.tiles_n = static_cast<int>(ceil_div(n, p.tile)), p.tiles_k = static_cast<int>(std::max<int64_t>(1, ceil_div(k, p.tile)));
-  const int64_t step = wgrad_step(dtype, p.tile), tiles = static_cast<int64_t>(p.tiles_n) * p.tiles_k;
-  const int64_t slots = kCus * (p.tile == 256 ? 1 : 2);
+  p.wide = ceil_div(n, 256) * ceil_div(k, 256) * 4 >= kCus;
+  const int64_t tn = p.wide ? WgradWide::kTileN : WgradSmall::kTileN, tk = p.wide ? WgradWide::kTileK : WgradSmall::kTileK;
+  p.tiles_n = static_cast<int>(ceil_div(n, tn)), p.tiles_k = static_cast<int>(std::max<int64_t>(1, ceil_div(k, tk)));
+  const int64_t step = p.wide ? WgradWide::step(dtype) : WgradSmall::step(dtype);
+  const int64_t tiles = static_cast<int64_t>(p.tiles_n) * p.tiles_k;
+  const int64_t slots = kCus * (p.wide ? 1 : 2);
   int64_t splits = std::max<int64_t>(1, slots / tiles);
   splits = std::min(splits, std::max<int64_t>(1, rows / (4 * step)));
   p.split_rows = round_up(ceil_div(std::max<int64_t>(rows, 1), splits), step);
@@ -371,11 +401,11 @@ static WgradPlan wgrad_plan(int dtype, int64_t rows, int64_t n, int64_t k) {
 }
 
 template <int DT, int FMT>
-static void wgrad_launch(const WgradArgs &a, int tile, dim3 grid, hipStream_t st) {
-  if (tile == 256) {
-    hipLaunchKernelGGL((wgrad_kernel<DT, FMT, 256>), grid, dim3(kWgThreads), 0, st, a);
+static void wgrad_launch(const WgradArgs &a, bool wide, dim3 grid, hipStream_t st) {
+  if (wide) {
+    hipLaunchKernelGGL((wgrad_kernel<DT, FMT, WgradWide>), grid, dim3(WgradWide::kThreads), 0, st, a);
   } else {
-    hipLaunchKernelGGL((wgrad_kernel<DT, FMT, 128>), grid, dim3(kWgThreads), 0, st, a);
+    hipLaunchKernelGGL((wgrad_kernel<DT, FMT, WgradSmall>), grid, dim3(WgradSmall::kThreads), 0, st, a);
   }
 }
 
@@ -386,7 +416,9 @@ using namespace smx;
 extern "C" int64_t smx_act8_wgrad_workspace_bytes(int64_t rows, int64_t n, int64_t k, int dtype) {
   if (rows < 0 || n < 0 || k < 0 || dtype < SMX_F32 || dtype > SMX_F16) return SMX_EINVAL;
   const WgradPlan p = wgrad_plan(dtype, rows, n, k);
-  return p.splits == 1 ? 0 : round_up(p.splits * (n * k + n) * static_cast<int64_t>(sizeof(float)), 256);
+  // the splits' partial tiles where there are several, and the parts of db
+  const int64_t tiles = p.splits > 1 ? p.splits * n * k : 0, db = static_cast<int64_t>(p.splits) * p.tiles_k * n;
+  return round_up((tiles + db) * static_cast<int64_t>(sizeof(float)), 256);
 }
 
 extern "C" int smx_act8_wgrad(const void *delta, int dtype, int64_t rows, int64_t n, int64_t delta_stride,
@@ -412,31 +444,31 @@ extern "C" int smx_act8_wgrad(const void *delta, int dtype, int64_t rows, int64_
               "act8_wgrad: workspace must be 256-byte aligned");
   const WgradPlan p = wgrad_plan(dtype, rows, n, k);
   WgradArgs a{};
-  a.delta = delta, a.codes = codes, a.scales = scales, a.dw = dw, a.db = db;
+  a.delta = delta, a.codes = codes, a.scales = scales, a.dw = dw;
   a.rows = rows, a.n = n, a.k = k, a.pitch = pitch, a.delta_stride = delta_stride;
   a.split_rows = p.split_rows, a.tiles_k = p.tiles_k, a.tiles = p.tiles_n * p.tiles_k, a.splits = p.splits, a.out = out_dtype;
-  if (p.splits > 1) {
-    a.dw = workspace, a.out = SMX_F32;
-    if (db) a.db = static_cast<float *>(workspace) + p.splits * n * k;
-  }
+  const int64_t tiles = p.splits > 1 ? p.splits * n * k : 0;
+  if (p.splits > 1) a.dw = workspace, a.out = SMX_F32;
+  if (db) a.db = static_cast<float *>(workspace) + tiles;
   const dim3 grid(static_cast<unsigned>(round_up(static_cast<int64_t>(a.tiles) * a.splits, 8)));
   const auto st = static_cast<hipStream_t>(stream);
   const bool i8 = fmt == SMX_ACT8_INT8;
   if (dtype == SMX_F32) {
-    i8 ? wgrad_launch<SMX_F32, SMX_ACT8_INT8>(a, p.tile, grid, st) : wgrad_launch<SMX_F32, SMX_ACT8_E4M3>(a, p.tile, grid, st);
+    i8 ? wgrad_launch<SMX_F32, SMX_ACT8_INT8>(a, p.wide, grid, st) : wgrad_launch<SMX_F32, SMX_ACT8_E4M3>(a, p.wide, grid, st);
   } else if (dtype == SMX_BF16) {
-    i8 ? wgrad_launch<SMX_BF16, SMX_ACT8_INT8>(a, p.tile, grid, st)
-       : wgrad_launch<SMX_BF16, SMX_ACT8_E4M3>(a, p.tile, grid, st);
+    i8 ? wgrad_launch<SMX_BF16, SMX_ACT8_INT8>(a, p.wide, grid, st)
+       : wgrad_launch<SMX_BF16, SMX_ACT8_E4M3>(a, p.wide, grid, st);
   } else {
-    i8 ? wgrad_launch<SMX_F16, SMX_ACT8_INT8>(a, p.tile, grid, st) : wgrad_launch<SMX_F16, SMX_ACT8_E4M3>(a, p.tile, grid, st);
+    i8 ? wgrad_launch<SMX_F16, SMX_ACT8_INT8>(a, p.wide, grid, st) : wgrad_launch<SMX_F16, SMX_ACT8_E4M3>(a, p.wide, grid, st);
   }
-  if (p.splits > 1) {
+  if (p.splits > 1 || db) {
     const int rc = check_launch("act8_wgrad");
     if (rc != SMX_OK) return rc;
-    const int64_t count = n * k;
-    hipLaunchKernelGGL(wgrad_join_kernel, dim3(static_cast<unsigned>(std::max(ceil_div(count, 1024), ceil_div(n, 256)))),
-                       dim3(256), 0, st, static_cast<const float *>(workspace), count, p.splits, dw, out_dtype,
-                       static_cast<const float *>(a.db), n, db);
+    const int64_t count = p.splits > 1 ? n * k : 0, blocks = ceil_div(count, 1024) + (db ? ceil_div(n, 16) : 0);
+    if (blocks == 0) return SMX_OK;
+    hipLaunchKernelGGL(wgrad_join_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st,
+                       static_cast<const float *>(workspace), count, p.splits, dw, out_dtype, a.db, n,
+                       p.splits * p.tiles_k, db);
   }
   return check_launch("act8_wgrad");
 }
