@@ -15,6 +15,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace smx {
 
@@ -92,9 +93,10 @@ __device__ __forceinline__ void store4(void *p, int64_t i, const float *v) {
   if constexpr (DT == SMX_F32) {
     *reinterpret_cast<float4 *>(static_cast<float *>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
   } else {
-    uint2 w;
-    store_any(&w, DT, 0, v[0]), store_any(&w, DT, 1, v[1]), store_any(&w, DT, 2, v[2]), store_any(&w, DT, 3, v[3]);
-    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + i) = w;
+    typedef std::conditional_t<DT == SMX_BF16, __bf16, _Float16> T;
+    typedef T v4t __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<v4t *>(static_cast<uint16_t *>(p) + i) =
+        v4t{static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
   }
 }
 
@@ -203,8 +205,6 @@ __global__ void __launch_bounds__(kQkThreads) qk_kernel(QkArgs a) {
       for (int k = 0; k < 8; ++k) y[k] = r * (g[k] - x[k] * dot);
     }
     if (l.active) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] = round_to(DT, y[k]);
       const int64_t at = qk_at(s.ys, it);
       store4<DT>(s.y, at + l.lo, y);
       store4<DT>(s.y, at + l.hi, y + 4);
@@ -293,25 +293,39 @@ __global__ void __launch_bounds__(kQkThreads) qk_any_kernel(QkArgs a, int half) 
   }
 }
 
-// dw[e] = sum over the partial rows, in FP64 and a fixed order; one block a
-// side and 64 elements.
+// dw[e] = sum over the partial rows, in FP64 and a fixed order: a block per side
+// and 16 elements, each from 64 threads.
 struct QkDwArgs {
   const float *part[2];
   void *dw[2];
   int32_t rows[2], dtype[2], dim;
 };
 __global__ void __launch_bounds__(1024) qk_dw_kernel(QkDwArgs a) {
-  __shared__ double red[16][64];
-  const int which = blockIdx.y, e = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
+  __shared__ double red[64][17];
+  const int which = blockIdx.y, col = threadIdx.x & 15, q = threadIdx.x >> 4, e = blockIdx.x * 16 + col;
   const float *part = a.part[which];
   if (!a.dw[which]) return;
   double t = 0;
-  if (e < a.dim)
-    for (int r = wave; r < a.rows[which]; r += 16) t += part[static_cast<int64_t>(r) * a.dim + e];
-  red[wave][threadIdx.x & 63] = t;
+  if (e < a.dim) {
+    int r = q;
+    for (; r + 7 * 64 < a.rows[which]; r += 8 * 64) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = part[static_cast<int64_t>(r + 64 * k) * a.dim + e];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t += v[k];
+    }
+    for (; r < a.rows[which]; r += 64) t += part[static_cast<int64_t>(r) * a.dim + e];
+  }
+  red[q][col] = t;
   __syncthreads();
-  if (wave == 0 && e < a.dim) {
-    for (int q = 1; q < 16; ++q) t += red[q][threadIdx.x & 63];
+  if (q < 8) {
+    for (int k = 1; k < 8; ++k) t += red[q + 8 * k][col];
+    red[q][col] = t;
+  }
+  __syncthreads();
+  if (q == 0 && e < a.dim) {
+    for (int k = 1; k < 8; ++k) t += red[k][col];
     store_any(a.dw[which], a.dtype[which], e, round_to(a.dtype[which], static_cast<float>(t)));
   }
 }
@@ -503,6 +517,6 @@ extern "C" int smx_qk_norm_rotary_backward(const smx_qk_desc *desc, void *worksp
     w.part[i] = part[i], w.dw[i] = s.dw, w.rows[i] = p.rows[i], w.dtype[i] = s.weight_dtype;
   }
   w.dim = static_cast<int32_t>(desc->dim);
-  hipLaunchKernelGGL(qk_dw_kernel, dim3(static_cast<unsigned>(ceil_div(desc->dim, 64)), 2), dim3(1024), 0, st, w);
+  hipLaunchKernelGGL(qk_dw_kernel, dim3(static_cast<unsigned>(ceil_div(desc->dim, 16)), 2), dim3(1024), 0, st, w);
   return check_launch("qk_norm_rotary_backward");
 }
