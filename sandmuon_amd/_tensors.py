@@ -1,4 +1,4 @@
-"""Argument checks shared by the operators of a training step (act8,
+"""Argument checks and calls shared by the operators of a training step (act8,
 attention, losses)."""
 from __future__ import annotations
 
@@ -8,23 +8,26 @@ import torch
 
 from . import _native
 
-FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_CODES = _native._DTYPES
+_current_device = torch._C._cuda_getDevice
 
 
 def need_float(t: torch.Tensor, what: str) -> torch.Tensor:
     """t, a GPU tensor of one of the three float types."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
-    _native.require_gpu(t, what)
-    if t.dtype not in FLOATS:
+    if not t.is_cuda:
+        _native.require_gpu(t, what)
+    if t.dtype not in _CODES:
         raise ValueError(f"{what}: unsupported dtype {t.dtype}; expected float32, bfloat16 or float16")
     return t
 
 
 def same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    device = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
 
 
 def unit_last(t: torch.Tensor) -> torch.Tensor:
@@ -40,19 +43,15 @@ def rows2d(t: torch.Tensor) -> torch.Tensor:
     return unit_last(t)
 
 
-class on_device:
-    """Makes t's device current for a launch, where it is not already."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, t: torch.Tensor):
-        index = t.device.index
-        self.guard = None if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def launch(name: str, device: torch.device, *args) -> None:
+    """Calls entry point `name` with `args` and the current stream of `device`,
+    which is made current for the call where it is not."""
+    fn = getattr(_native.lib(), name)
+    index = device.index
+    if index == _current_device():
+        rc = fn(*args, _native.stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _native.stream_of(device))
+    if rc != 0:
+        _native._check(rc, name)

@@ -36,7 +36,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from ._tensors import need_float, on_device, rows2d, same_device
+from ._tensors import launch, need_float, rows2d, same_device
 
 __all__ = ["Act8", "FORMATS", "checkpoint_linears", "decode", "encode", "gelu", "gelu_backward", "gelu_forward",
            "linear", "linear_backward", "mlp"]
@@ -58,13 +58,13 @@ class Act8:
 
     __slots__ = ("data", "shape", "rows", "cols", "pitch", "fmt")
 
-    def __init__(self, shape, fmt: str, device):
-        self.shape = torch.Size(shape)
-        self.cols = self.shape[-1]
-        self.rows = self.shape[:-1].numel()
-        self.pitch = -(-self.cols // _BLOCK) * _BLOCK
+    def __init__(self, shape: torch.Size, fmt: str, device):
+        self.shape = shape
+        self.cols = shape[-1]
+        self.rows = rows = shape[0] if len(shape) == 2 else shape[:-1].numel()
+        self.pitch = pitch = -(-shape[-1] // _BLOCK) * _BLOCK
         self.fmt = fmt
-        self.data = torch.empty(self.rows * (self.pitch + self.pitch // _BLOCK), dtype=torch.uint8, device=device)
+        self.data = torch.empty(rows * (pitch + pitch // _BLOCK), dtype=torch.uint8, device=device)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -87,7 +87,7 @@ def _activation(x: torch.Tensor, what: str) -> torch.Tensor:
     need_float(x, what)
     if x.dim() < 1:
         raise ValueError(f"{what}: expected at least one dimension")
-    return x.detach()
+    return x.detach() if x.requires_grad else x
 
 
 def _kept(saved: Act8, what: str) -> Act8:
@@ -103,10 +103,8 @@ def encode(x: torch.Tensor, fmt: str = "int8") -> Act8:
     rows = rows2d(x)
     saved = Act8(x.shape, fmt, x.device)
     codes, scales = saved._ptrs()
-    with on_device(rows):
-        _native._check(_native.lib().smx_act8_encode(
-            rows.data_ptr(), _native.dtype_code(rows.dtype), saved.rows, saved.cols, rows.stride(0), code, codes,
-            scales, saved.pitch, _native.stream_of(rows.device)), "smx_act8_encode")
+    launch("smx_act8_encode", rows.device, rows.data_ptr(), _native.dtype_code(rows.dtype), saved.rows, saved.cols,
+           rows.stride(0), code, codes, scales, saved.pitch)
     return saved
 
 
@@ -115,10 +113,8 @@ def decode(saved: Act8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     _kept(saved, "act8.decode")
     out = torch.empty(saved.shape, dtype=dtype, device=saved.data.device)
     codes, scales = saved._ptrs()
-    with on_device(out):
-        _native._check(_native.lib().smx_act8_decode(
-            codes, scales, FORMATS[saved.fmt], saved.rows, saved.cols, saved.pitch, out.data_ptr(),
-            _native.dtype_code(dtype), saved.cols, _native.stream_of(out.device)), "smx_act8_decode")
+    launch("smx_act8_decode", out.device, codes, scales, FORMATS[saved.fmt], saved.rows, saved.cols, saved.pitch,
+           out.data_ptr(), _native.dtype_code(dtype), saved.cols)
     return out
 
 
@@ -131,11 +127,9 @@ def gelu_forward(h: torch.Tensor, fmt: str = "int8",
     y = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     kept_h = Act8(h.shape, fmt, h.device)
     kept_y = Act8(h.shape, fmt, h.device) if keep_output else None
-    with on_device(rows):
-        _native._check(_native.lib().smx_act8_gelu(
-            rows.data_ptr(), _native.dtype_code(h.dtype), kept_h.rows, kept_h.cols, rows.stride(0), code, y.data_ptr(),
-            kept_h.cols, *kept_h._ptrs(), *(kept_y._ptrs() if keep_output else (None, None)), kept_h.pitch,
-            _native.stream_of(rows.device)), "smx_act8_gelu")
+    launch("smx_act8_gelu", rows.device, rows.data_ptr(), _native.dtype_code(h.dtype), kept_h.rows, kept_h.cols,
+           rows.stride(0), code, y.data_ptr(), kept_h.cols, *kept_h._ptrs(), *(kept_y._ptrs() if keep_output else
+           (None, None)), kept_h.pitch)
     return y, kept_h, kept_y
 
 
@@ -149,11 +143,8 @@ def gelu_backward(dy: torch.Tensor, saved: Act8) -> torch.Tensor:
     rows = rows2d(dy)
     dh = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
     codes, scales = saved._ptrs()
-    with on_device(rows):
-        _native._check(_native.lib().smx_act8_gelu_backward(
-            rows.data_ptr(), _native.dtype_code(dy.dtype), saved.rows, saved.cols, rows.stride(0), codes, scales,
-            FORMATS[saved.fmt], saved.pitch, dh.data_ptr(), saved.cols, _native.stream_of(rows.device)),
-            "smx_act8_gelu_backward")
+    launch("smx_act8_gelu_backward", rows.device, rows.data_ptr(), _native.dtype_code(dy.dtype), saved.rows,
+           saved.cols, rows.stride(0), codes, scales, FORMATS[saved.fmt], saved.pitch, dh.data_ptr(), saved.cols)
     return dh
 
 
@@ -178,11 +169,8 @@ def linear_backward(delta: torch.Tensor, saved: Act8, dtype: Optional[torch.dtyp
     need = lib.smx_act8_wgrad_workspace_bytes(saved.rows, n, saved.cols, code)
     work = torch.empty(need, dtype=torch.uint8, device=delta.device) if need else None
     codes, scales = saved._ptrs()
-    with on_device(rows):
-        _native._check(lib.smx_act8_wgrad(
-            rows.data_ptr(), code, saved.rows, n, rows.stride(0), codes, scales, FORMATS[saved.fmt], saved.cols,
-            saved.pitch, dw.data_ptr(), _native.ptr(db), out, _native.ptr(work), need,
-            _native.stream_of(rows.device)), "smx_act8_wgrad")
+    launch("smx_act8_wgrad", rows.device, rows.data_ptr(), code, saved.rows, n, rows.stride(0), codes, scales,
+           FORMATS[saved.fmt], saved.cols, saved.pitch, dw.data_ptr(), _native.ptr(db), out, _native.ptr(work), need)
     return dw, db
 
 

@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from ._tensors import need_float, on_device, same_device, unit_last
+from ._tensors import launch, need_float, same_device, unit_last
 
 __all__ = ["qk_norm_rotary", "rotary_tables"]
 
@@ -56,8 +56,7 @@ def _forward(q, k, qw, kw, cos, sin, positions, position0, eps, style, out):
         out = (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device))
     desc = _desc(_side(q, qw, None, out[0], None), _side(k, kw, None, out[1], None), q, cos, sin, positions, position0,
                  eps, style)
-    with on_device(q):
-        _native._check(_native.lib().smx_qk_norm_rotary(desc, _native.stream_of(q.device)), "smx_qk_norm_rotary")
+    launch("smx_qk_norm_rotary", q.device, desc)
     return out
 
 
@@ -87,14 +86,10 @@ class _QkNormRotary(torch.autograd.Function):
             sides.append(_side(x, w, dy, dx, dw))
             grads.append((dx if need_x else None, dw, dy))
         if any(s[5] for s in sides):
-            lib = _native.lib()
-            need = lib.smx_qk_workspace_bytes(q.shape[3]) if needs[2] or needs[3] else 0
+            need = _native.lib().smx_qk_workspace_bytes(q.shape[3]) if needs[2] or needs[3] else 0
             work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
             desc = _desc(*sides, q, cos, sin, positions, position0, eps, style)
-            with on_device(q):
-                _native._check(lib.smx_qk_norm_rotary_backward(desc, _native.ptr(work), need,
-                                                               _native.stream_of(q.device)),
-                               "smx_qk_norm_rotary_backward")
+            launch("smx_qk_norm_rotary_backward", q.device, desc, _native.ptr(work), need)
         return grads[0][0], grads[1][0], grads[0][1], grads[1][1], None, None, None, None, None, None
 
 

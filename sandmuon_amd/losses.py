@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from ._tensors import need_float, on_device, same_device, unit_last
+from ._tensors import launch, need_float, same_device, unit_last
 
 __all__ = ["policy_loss", "preference_loss", "token_logprobs"]
 
@@ -58,18 +58,14 @@ def _rows(logits, targets, mask):
 def _logprobs(logits, targets, mask, want_stats):
     lp = torch.empty(targets.shape, dtype=torch.float32, device=logits.device)
     stats = torch.empty(*targets.shape, 2, dtype=torch.float32, device=logits.device) if want_stats else None
-    with on_device(logits):
-        _native._check(_native.lib().smx_token_logprobs(*_rows(logits, targets, mask), lp.data_ptr(), _native.ptr(stats),
-                                                        _native.stream_of(logits.device)), "smx_token_logprobs")
+    launch("smx_token_logprobs", logits.device, *_rows(logits, targets, mask), lp.data_ptr(), _native.ptr(stats))
     return lp, stats
 
 
 def _logprobs_backward(logits, targets, mask, stats, coef, strides, scale):
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    with on_device(logits):
-        _native._check(_native.lib().smx_token_logprobs_backward(
-            *_rows(logits, targets, mask), stats.data_ptr(), coef.data_ptr(), *strides, _native.ptr(scale),
-            out.data_ptr(), _native.stream_of(logits.device)), "smx_token_logprobs_backward")
+    launch("smx_token_logprobs_backward", logits.device, *_rows(logits, targets, mask), stats.data_ptr(),
+           coef.data_ptr(), *strides, _native.ptr(scale), out.data_ptr())
     return out
 
 
@@ -106,11 +102,9 @@ class _PolicyLoss(torch.autograd.Function):
         lib = _native.lib()
         need = lib.smx_policy_loss_workspace_bytes(*targets.shape)
         work = torch.empty(need, dtype=torch.uint8, device=device)
-        with on_device(logits):
-            _native._check(lib.smx_policy_loss(
-                *_rows(logits, targets, mask), _native.ptr(old), _native.ptr(ref), adv.data_ptr(), *adv_strides, low,
-                high, kl, reduction, scale, loss.data_ptr(), lp.data_ptr(), _native.ptr(grad), work.data_ptr(), need,
-                _native.stream_of(device)), "smx_policy_loss")
+        launch("smx_policy_loss", logits.device, *_rows(logits, targets, mask), _native.ptr(old), _native.ptr(ref),
+               adv.data_ptr(), *adv_strides, low, high, kl, reduction, scale, loss.data_ptr(), lp.data_ptr(),
+               _native.ptr(grad), work.data_ptr(), need)
         ctx.grad = grad
         ctx.mark_non_differentiable(lp)
         return loss, lp
@@ -123,9 +117,8 @@ class _PolicyLoss(torch.autograd.Function):
             raise RuntimeError("policy_loss: the gradient is made with the loss and handed out once; "
                                "call policy_loss again to go through it a second time")
         grad_loss = grad_loss.float()
-        with on_device(grad):
-            _native._check(_native.lib().smx_scale(grad.data_ptr(), _native.dtype_code(grad.dtype), grad.numel(),
-                                                   grad_loss.data_ptr(), _native.stream_of(grad.device)), "smx_scale")
+        launch("smx_scale", grad.device, grad.data_ptr(), _native.dtype_code(grad.dtype), grad.numel(),
+               grad_loss.data_ptr())
         return (grad,) + (None,) * 11
 
 
@@ -177,11 +170,8 @@ class _PreferenceLoss(torch.autograd.Function):
         loss = torch.empty((), dtype=torch.float32, device=device)
         margins = torch.empty(pairs, dtype=torch.float32, device=device)
         coef = torch.empty(2 * pairs, dtype=torch.float32, device=device)
-        with on_device(logits):
-            _native._check(_native.lib().smx_preference_loss(
-                lp.data_ptr(), ref.data_ptr(), _native.ptr(mask), pairs, logits.shape[1], beta, smoothing,
-                loss.data_ptr(), margins.data_ptr(), coef.data_ptr(), _native.stream_of(device)),
-                "smx_preference_loss")
+        launch("smx_preference_loss", logits.device, lp.data_ptr(), ref.data_ptr(), _native.ptr(mask), pairs,
+               logits.shape[1], beta, smoothing, loss.data_ptr(), margins.data_ptr(), coef.data_ptr())
         if stats is not None:
             ctx.save_for_backward(logits, targets, mask, stats, coef)
         ctx.mark_non_differentiable(margins)
