@@ -37,14 +37,16 @@ struct WgradArgs {
 
 constexpr int parts_of(int dt) { return dt == SMX_BF16 ? 1 : dt == SMX_F16 ? 2 : 3; }
 
-// Tiles: rows and columns, the waves that share them, and the rows of a step.
-template <int TN, int TK, int WN, int WK, int STEP, int STEP_PARTS, int WPS>
+// Tiles: rows and columns, the waves that share them, the rows of a step, and
+// where in a step the next one is staged (MID: between its halves).
+template <int TN, int TK, int WN, int WK, int STEP, int STEP_PARTS, int WPS, bool MID>
 struct WgradTile {
+  static constexpr bool kMid = MID;
   static constexpr int kTileN = TN, kTileK = TK, kWavesN = WN, kWavesK = WK, kThreads = 64 * WN * WK, kWavesPerSimd = WPS;
   static constexpr int step(int dt) { return dt == SMX_BF16 ? STEP : STEP_PARTS; }
 };
-using WgradWide = WgradTile<256, 256, 2, 4, 64, 32, 2>;
-using WgradSmall = WgradTile<128, 128, 2, 2, 64, 32, 2>;
+using WgradWide = WgradTile<256, 256, 2, 4, 64, 32, 2, true>;
+using WgradSmall = WgradTile<128, 128, 2, 2, 64, 32, 2, false>;
 
 // 16 codes and their scale to 16 BF16 values (two uint4).
 template <int FMT>
@@ -257,17 +259,24 @@ __global__ void __launch_bounds__(C::kThreads, C::kWavesPerSimd) wgrad_kernel(Wg
 #pragma unroll
     for (int i = 0; i < kCodeLoads; ++i) stage_codes(to, i);
   };
+  // The next step's registers are staged between the halves of a step, where
+  // one block has the CU to itself (two waves a SIMD): what one wave stages,
+  // the other covers with MFMAs.  Where two blocks share it, they do that for
+  // each other, and staging behind a step's MFMAs leaves its loads more time.
+  // (8192 x 2048 x 8192 e4m3, wide: 252 us, 265 us behind; 16384 x 768 x 768,
+  // small: 42 us, 39 us behind.)
   if (steps > 0) {
     load(0);
     add_bias(0);
     stage(lds);
+    if (C::kMid && steps > 1) load(1);
   }
   __syncthreads();
+  constexpr int kHalf = kStep / 32;
   for (int t = 0; t < steps; ++t) {
     const char *at = lds + (t & 1) * kBuffer;
-    if (t + 1 < steps) load(t + 1);
-#pragma unroll
-    for (int ms = 0; ms < kStep / 16; ++ms) {
+    char *next = lds + ((t & 1) ^ 1) * kBuffer;
+    const auto products = [&](int ms) __attribute__((always_inline)) {
       v8bf bv[FK];
 #pragma unroll
       for (int h = 0; h < FK; ++h) bv[h] = operand(at + ms * 16 * 2 * TK + b_at[h], 4 * 2 * TK);
@@ -279,10 +288,21 @@ __global__ void __launch_bounds__(C::kThreads, C::kWavesPerSimd) wgrad_kernel(Wg
 #pragma unroll
           for (int h = 0; h < FK; ++h) acc[f][h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av, bv[h], acc[f][h], 0, 0, 0);
         }
+    };
+    if (!C::kMid && t + 1 < steps) load(t + 1);
+#pragma unroll
+    for (int ms = 0; ms < kHalf; ++ms) products(ms);
+    if constexpr (C::kMid) {
+      // (the last step stages registers that nobody reads)
+      if (t + 1 < steps) add_bias(t + 1);
+      stage(next);
+      if (t + 2 < steps) load(t + 2);
     }
-    if (t + 1 < steps) {
+#pragma unroll
+    for (int ms = kHalf; ms < kStep / 16; ++ms) products(ms);
+    if (!C::kMid && t + 1 < steps) {
       add_bias(t + 1);
-      stage(lds + ((t & 1) ^ 1) * kBuffer);
+      stage(next);
     }
     __syncthreads();
   }
@@ -382,22 +402,39 @@ struct WgradPlan {
   int64_t split_rows;
 };
 
-// 256 x 256 tiles (one block per CU) where they fill the CUs with few splits;
-// 128 x 128 tiles (two blocks per CU) otherwise.
+// The tile and the splits of the rows with the least expected time:
+//   steps of 64 rows times what a step takes a CU (BF16 cotangents, measured:
+//   2.0 us a wide tile, 1.2 us a small one alone on its CU, 1.6 us two small
+//   ones together; each further part of the cotangents adds 0.8 of that), 7 or
+//   2.5 us for a wide or small tile's first loads and last stores, and where
+//   the rows are split the join's launch (4 us) and the partial tiles at 8 TB/s
+//   written and read.
+// (Measured on either tile: 2048 x 2048 x 2048 e4m3 45 us wide, 35 us small;
+// 16384 x 768 x 3072 93 us wide, 110 us small; 64 x 2048 x 2048 16 and 10 us.)
 static WgradPlan wgrad_plan(int dtype, int64_t rows, int64_t n, int64_t k) {
-  WgradPlan p{};
   constexpr int64_t kCus = 256;
-  p.wide = ceil_div(n, 256) * ceil_div(k, 256) * 4 >= kCus;
-  const int64_t tn = p.wide ? WgradWide::kTileN : WgradSmall::kTileN, tk = p.wide ? WgradWide::kTileK : WgradSmall::kTileK;
-  p.tiles_n = static_cast<int>(ceil_div(n, tn)), p.tiles_k = static_cast<int>(std::max<int64_t>(1, ceil_div(k, tk)));
-  const int64_t step = p.wide ? WgradWide::step(dtype) : WgradSmall::step(dtype);
-  const int64_t tiles = static_cast<int64_t>(p.tiles_n) * p.tiles_k;
-  const int64_t slots = kCus * (p.wide ? 1 : 2);
-  int64_t splits = std::max<int64_t>(1, slots / tiles);
-  splits = std::min(splits, std::max<int64_t>(1, rows / (4 * step)));
-  p.split_rows = round_up(ceil_div(std::max<int64_t>(rows, 1), splits), step);
-  p.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(rows, p.split_rows)));
-  return p;
+  WgradPlan best{};
+  double best_us = 0;
+  for (const bool wide : {true, false}) {
+    const int64_t tn = wide ? WgradWide::kTileN : WgradSmall::kTileN, tk = wide ? WgradWide::kTileK : WgradSmall::kTileK;
+    const int64_t tiles_n = ceil_div(n, tn), tiles_k = std::max<int64_t>(1, ceil_div(k, tk)), tiles = tiles_n * tiles_k;
+    const int64_t step = wide ? WgradWide::step(dtype) : WgradSmall::step(dtype);
+    const int64_t most = std::min<int64_t>(64, std::max<int64_t>(1, 2 * kCus / tiles));
+    for (int64_t s = 1; s <= most; ++s) {
+      const int64_t split_rows = round_up(ceil_div(std::max<int64_t>(rows, 1), s), step);
+      if (s > 1 && ceil_div(rows, split_rows) != s) continue;  // (as many splits with fewer rows each came before)
+      const int64_t per_cu = ceil_div(tiles * s, kCus);
+      const double steps = static_cast<double>(split_rows) / 64 * (0.2 + 0.8 * parts_of(dtype));
+      const double small = per_cu == 1 ? 1.2 : 1.6 * static_cast<double>(ceil_div(per_cu, 2));
+      double us = steps * (wide ? 2.0 * static_cast<double>(per_cu) : small) + (wide ? 7 : 2.5);
+      if (s > 1) us += 4 + static_cast<double>(s * n * k) * 8 / 8e6;
+      if (best_us == 0 || us < best_us) {
+        best_us = us;
+        best = {wide, static_cast<int>(tiles_n), static_cast<int>(tiles_k), static_cast<int>(s), split_rows};
+      }
+    }
+  }
+  return best;
 }
 
 template <int DT, int FMT>
