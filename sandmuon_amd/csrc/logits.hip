@@ -421,26 +421,53 @@ struct PreferenceArgs {
 };
 
 // The gain of each sequence (sum of its live log ratios) in FP64, then a
-// pair's margin, loss and d loss / d lp: a wave a pair, one block.
-__global__ void __launch_bounds__(1024) preference_kernel(PreferenceArgs a) {
-  __shared__ double scratch[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// pair's margin, loss and d loss / d lp.  One block of 16 waves, `share` of them
+// (a power of two) to a pair, four tokens of each lane in flight at once.
+__global__ void __launch_bounds__(1024) preference_kernel(PreferenceArgs a, int share) {
+  __shared__ double scratch[16], part[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lead = wave / share * share;
   double loss = 0;
-  for (int64_t p = wave; p < a.pairs; p += 16) {
+  for (int64_t p0 = 0; p0 < a.pairs; p0 += 16 / share) {
+    const int64_t p = p0 + wave / share;
     double gain = 0;
-    for (int side = 0; side < 2; ++side) {
-      const int64_t at = (p + side * a.pairs) * a.seq;
-      double g = 0;
-      for (int64_t t = lane; t < a.seq; t += 64)
-        if (!a.mask || a.mask[at + t]) g += static_cast<double>(a.lp[at + t]) - a.ref[at + t];
-      gain += side ? -g : g;
+    if (p < a.pairs) {
+      const int64_t at[2] = {p * a.seq, (p + a.pairs) * a.seq};
+      for (int64_t t0 = (wave - lead) * 64 + lane; t0 < a.seq; t0 += 4 * 64 * share) {
+        // (what a masked token's ref holds is loaded, not used)
+        float lp[2][4], ref[2][4];
+        bool live[2][4];
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int64_t t = t0 + u * 64 * share, i = at[side] + (t < a.seq ? t : t0);
+            live[side][u] = t < a.seq && (!a.mask || a.mask[i]);
+            lp[side][u] = a.lp[i], ref[side][u] = a.ref[i];
+          }
+        double g[2];
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+          float d[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) d[u] = live[side][u] ? lp[side][u] - ref[side][u] : 0.f;
+          g[side] = (static_cast<double>(d[0]) + d[1]) + (static_cast<double>(d[2]) + d[3]);
+        }
+        gain += g[0] - g[1];
+      }
     }
-    const double m = a.beta * wave_sum(gain);
-    const double soft = log1p(exp(-fabs(m)));
-    if (lane == 0) {
-      loss += (1 - a.smoothing) * (soft - fmin(m, 0.)) + a.smoothing * (soft + fmax(m, 0.));
-      a.margins[p] = static_cast<float>(m);
-      const double slope = a.beta * (1 / (1 + exp(-m)) - (1 - a.smoothing)) / a.pairs;
+    gain = wave_sum(gain);
+    __syncthreads();
+    if (lane == 0) part[wave] = gain;
+    __syncthreads();
+    if (p < a.pairs && wave == lead && lane == 0) {
+      for (int w = 1; w < share; ++w) gain += part[lead + w];
+      // (the margin is rounded once; FP32 functions of it are within 2^-22)
+      const float m = static_cast<float>(a.beta * gain), e = expf(-fabsf(m)), soft = log1pf(e);
+      loss += (1 - a.smoothing) * (soft - (m > 0.f ? 0.f : m)) + a.smoothing * (soft + (m < 0.f ? 0.f : m));
+      a.margins[p] = m;
+      // sigmoid(m) = 1 / (1 + e) or e / (1 + e)
+      const double up = static_cast<double>(m > 0.f ? 1.f : e) / (1.0 + e);
+      const double slope = a.beta * (up - (1 - a.smoothing)) / a.pairs;
       a.coef[p] = static_cast<float>(slope);
       a.coef[p + a.pairs] = static_cast<float>(-slope);
     }
@@ -583,7 +610,9 @@ extern "C" int smx_preference_loss(const float *logprobs, const float *ref_logpr
   SMX_REQUIRE(loss && (pairs == 0 || (margins && coef)), SMX_EINVAL, "preference_loss: null output");
   SMX_REQUIRE(pairs == 0 || seq == 0 || (logprobs && ref_logprobs), SMX_EINVAL, "preference_loss: null log probabilities");
   const PreferenceArgs a{logprobs, ref_logprobs, mask, pairs, seq, beta, label_smoothing, loss, margins, coef};
-  hipLaunchKernelGGL(preference_kernel, dim3(1), dim3(1024), 0, static_cast<hipStream_t>(stream), a);
+  int share = 16;
+  while (share > 1 && 16 / share < pairs) share /= 2;
+  hipLaunchKernelGGL(preference_kernel, dim3(1), dim3(1024), 0, static_cast<hipStream_t>(stream), a, share);
   return check_launch("preference_loss");
 }
 
