@@ -29,69 +29,66 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return w;
 }
 
+template <int DT>
+__device__ __forceinline__ void unpack2(uint32_t w, float *v) {
+  if constexpr (DT == SMX_BF16) {
+    v[0] = __uint_as_float(w << 16);
+    v[1] = __uint_as_float(w & 0xffff0000u);
+  } else {
+    v[0] = f16_bits_to_f32(static_cast<uint16_t>(w));
+    v[1] = f16_bits_to_f32(static_cast<uint16_t>(w >> 16));
+  }
+}
+
 // Eight values as their type holds them.
 template <int DT>
 __device__ __forceinline__ void round8(float *v) {
   if constexpr (DT != SMX_F32) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t w = pack2<DT>(v[2 * k], v[2 * k + 1]);
-      if constexpr (DT == SMX_BF16) {
-        v[2 * k] = __uint_as_float(w << 16);
-        v[2 * k + 1] = __uint_as_float(w & 0xffff0000u);
-      } else {
-        v[2 * k] = f16_bits_to_f32(static_cast<uint16_t>(w));
-        v[2 * k + 1] = f16_bits_to_f32(static_cast<uint16_t>(w >> 16));
-      }
-    }
+    for (int k = 0; k < 4; ++k) unpack2<DT>(pack2<DT>(v[2 * k], v[2 * k + 1]), v + 2 * k);
   }
 }
 
-template <int DT, bool VEC>
+// 16 bytes at the elements' own alignment: rows of an odd width are read and
+// written like others.
+typedef uint32_t act8_v4u __attribute__((ext_vector_type(4), aligned(2)));
+
+template <int DT>
 struct Elems8 {
   // Elements [i, i + n) of p, n <= 8; the rest are zero.
   static __device__ __forceinline__ void load(const void *p, int64_t i, int n, float *v) {
-    if constexpr (VEC) {
-      if constexpr (DT == SMX_F32) {
-        const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
-        const float4 b = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-      } else {
-        const uint4 a = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if constexpr (DT == SMX_BF16) {
-            v[2 * k] = __uint_as_float(w[k] << 16);
-            v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-          } else {
-            v[2 * k] = f16_bits_to_f32(static_cast<uint16_t>(w[k]));
-            v[2 * k + 1] = f16_bits_to_f32(static_cast<uint16_t>(w[k] >> 16));
-          }
-        }
-      }
-    } else {
+    if (n < 8) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = k < n ? load_elem<DT>(p, i + k) : 0.f;
+      return;
+    }
+    if constexpr (DT == SMX_F32) {
+      const auto *at = reinterpret_cast<const act8_v4u *>(static_cast<const float *>(p) + i);
+      const act8_v4u a = at[0], b = at[1];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(a[k]), v[4 + k] = __uint_as_float(b[k]);
+    } else {
+      const act8_v4u a = *reinterpret_cast<const act8_v4u *>(static_cast<const uint16_t *>(p) + i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) unpack2<DT>(a[k], v + 2 * k);
     }
   }
   static __device__ __forceinline__ void store(void *p, int64_t i, int n, const float *v) {
-    if constexpr (VEC) {
-      if constexpr (DT == SMX_F32) {
-        float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(p) + i);
-        o[0] = make_float4(v[0], v[1], v[2], v[3]);
-        o[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = pack2<DT>(v[2 * k], v[2 * k + 1]);
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    } else {
+    if (n < 8) {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         if (k < n) store_any(p, DT, i + k, round_to(DT, v[k]));
+      return;
+    }
+    if constexpr (DT == SMX_F32) {
+      auto *at = reinterpret_cast<act8_v4u *>(static_cast<float *>(p) + i);
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        at[q] = act8_v4u{__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
+                         __float_as_uint(v[4 * q + 3])};
+    } else {
+      *reinterpret_cast<act8_v4u *>(static_cast<uint16_t *>(p) + i) =
+          act8_v4u{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7])};
     }
   }
 };
@@ -182,9 +179,9 @@ __device__ __forceinline__ float gelu_slope(float h) {
 
 enum Act8Op : int { kActEncode = 0, kActGelu = 1, kActDecode = 2, kActGeluBack = 3 };
 
-template <int DT, int FMT, int OP, bool VEC>
+template <int DT, int FMT, int OP>
 __global__ void __launch_bounds__(256) act8_kernel(Act8Args a) {
-  using E = Elems8<DT, VEC>;
+  using E = Elems8<DT>;
   const int chunk = blockIdx.x * blockDim.x + threadIdx.x;
   if (8 * static_cast<int64_t>(chunk) >= a.pitch) return;
   const int n = static_cast<int>(min<int64_t>(8, max<int64_t>(0, a.cols - 8 * static_cast<int64_t>(chunk))));
@@ -192,8 +189,7 @@ __global__ void __launch_bounds__(256) act8_kernel(Act8Args a) {
   for (int64_t r = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; r < a.rows; r += step) {
     float v[8] = {};
     if constexpr (OP == kActEncode || OP == kActGelu) {
-      // (whole groups of 8, or in the padding none: no load)
-      if (!VEC || n > 0) E::load(a.x, r * a.x_stride + 8 * chunk, n, v);
+      if (n > 0) E::load(a.x, r * a.x_stride + 8 * chunk, n, v);
       act8_put<FMT>(v, a.x8, r, a.pitch, chunk);
       if constexpr (OP == kActGelu) {
         // (the output is kept as it is stored: rounded to its type first)
@@ -220,39 +216,28 @@ __global__ void __launch_bounds__(256) act8_kernel(Act8Args a) {
 }
 
 template <int DT, int FMT, int OP>
-static int act8_launch_as(const Act8Args &a, bool vec, hipStream_t st, const char *what) {
+static int act8_launch_as(const Act8Args &a, hipStream_t st, const char *what) {
   const int64_t chunks = a.pitch / 8;
   const int64_t gx = ceil_div(chunks, 256);
   const int tx = static_cast<int>(round_up(ceil_div(chunks, gx), 4));
   const int ty = std::max(1, 256 / tx);
   const int64_t gy = std::min<int64_t>(ceil_div(a.rows, ty), 32768);
   const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), block(tx, ty);
-  if (vec) {
-    hipLaunchKernelGGL((act8_kernel<DT, FMT, OP, true>), grid, block, 0, st, a);
-  } else {
-    hipLaunchKernelGGL((act8_kernel<DT, FMT, OP, false>), grid, block, 0, st, a);
-  }
+  hipLaunchKernelGGL((act8_kernel<DT, FMT, OP>), grid, block, 0, st, a);
   return check_launch(what);
 }
 
 template <int OP>
-static int act8_launch(const Act8Args &a, int dtype, int fmt, bool vec, hipStream_t st, const char *what) {
+static int act8_launch(const Act8Args &a, int dtype, int fmt, hipStream_t st, const char *what) {
   const bool i8 = fmt == SMX_ACT8_INT8;
   if (dtype == SMX_F32)
-    return i8 ? act8_launch_as<SMX_F32, SMX_ACT8_INT8, OP>(a, vec, st, what)
-              : act8_launch_as<SMX_F32, SMX_ACT8_E4M3, OP>(a, vec, st, what);
+    return i8 ? act8_launch_as<SMX_F32, SMX_ACT8_INT8, OP>(a, st, what)
+              : act8_launch_as<SMX_F32, SMX_ACT8_E4M3, OP>(a, st, what);
   if (dtype == SMX_BF16)
-    return i8 ? act8_launch_as<SMX_BF16, SMX_ACT8_INT8, OP>(a, vec, st, what)
-              : act8_launch_as<SMX_BF16, SMX_ACT8_E4M3, OP>(a, vec, st, what);
-  return i8 ? act8_launch_as<SMX_F16, SMX_ACT8_INT8, OP>(a, vec, st, what)
-            : act8_launch_as<SMX_F16, SMX_ACT8_E4M3, OP>(a, vec, st, what);
-}
-
-// 16-byte loads and stores of 8 elements: every row starts on 16 bytes and
-// holds whole groups of 8 (padding groups are not touched).
-static bool act8_vec(const void *p, int dtype, int64_t cols, int64_t stride, int64_t rows) {
-  const int64_t e = dtype == SMX_F32 ? 4 : 2;
-  return cols % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || stride * e % 16 == 0);
+    return i8 ? act8_launch_as<SMX_BF16, SMX_ACT8_INT8, OP>(a, st, what)
+              : act8_launch_as<SMX_BF16, SMX_ACT8_E4M3, OP>(a, st, what);
+  return i8 ? act8_launch_as<SMX_F16, SMX_ACT8_INT8, OP>(a, st, what)
+            : act8_launch_as<SMX_F16, SMX_ACT8_E4M3, OP>(a, st, what);
 }
 
 static std::string act8_name(const char *what, const char *msg) { return std::string(what) + ": " + msg; }
@@ -299,8 +284,7 @@ extern "C" int smx_act8_encode(const void *x, int dtype, int64_t rows, int64_t c
   ACT8_TRY(act8_check_codes(what, codes, scales));
   Act8Args a{};
   a.x = x, a.x8 = {codes, scales}, a.rows = rows, a.cols = cols, a.pitch = pitch, a.x_stride = row_stride;
-  return act8_launch<kActEncode>(a, dtype, fmt, act8_vec(x, dtype, cols, row_stride, rows),
-                                 static_cast<hipStream_t>(stream), what);
+  return act8_launch<kActEncode>(a, dtype, fmt, static_cast<hipStream_t>(stream), what);
 }
 
 extern "C" int smx_act8_decode(const uint8_t *codes, const uint8_t *scales, int fmt, int64_t rows, int64_t cols,
@@ -313,8 +297,7 @@ extern "C" int smx_act8_decode(const uint8_t *codes, const uint8_t *scales, int 
   Act8Args a{};
   a.y = out, a.rows = rows, a.cols = cols, a.pitch = pitch, a.y_stride = out_stride;
   a.x8 = {const_cast<uint8_t *>(codes), const_cast<uint8_t *>(scales)};
-  return act8_launch<kActDecode>(a, dtype, fmt, act8_vec(out, dtype, cols, out_stride, rows),
-                                 static_cast<hipStream_t>(stream), what);
+  return act8_launch<kActDecode>(a, dtype, fmt, static_cast<hipStream_t>(stream), what);
 }
 
 extern "C" int smx_act8_gelu(const void *h, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int fmt, void *y,
@@ -332,8 +315,7 @@ extern "C" int smx_act8_gelu(const void *h, int dtype, int64_t rows, int64_t col
   Act8Args a{};
   a.x = h, a.y = y, a.x8 = {h_codes, h_scales}, a.y8 = {y_codes, y_scales};
   a.rows = rows, a.cols = cols, a.pitch = pitch, a.x_stride = row_stride, a.y_stride = y_stride;
-  const bool vec = act8_vec(h, dtype, cols, row_stride, rows) && act8_vec(y, dtype, cols, y_stride, rows);
-  return act8_launch<kActGelu>(a, dtype, fmt, vec, static_cast<hipStream_t>(stream), what);
+  return act8_launch<kActGelu>(a, dtype, fmt, static_cast<hipStream_t>(stream), what);
 }
 
 extern "C" int smx_act8_gelu_backward(const void *dy, int dtype, int64_t rows, int64_t cols, int64_t dy_stride,
@@ -348,6 +330,5 @@ extern "C" int smx_act8_gelu_backward(const void *dy, int dtype, int64_t rows, i
   Act8Args a{};
   a.dy = dy, a.y = dh, a.x8 = {const_cast<uint8_t *>(h_codes), const_cast<uint8_t *>(h_scales)};
   a.rows = rows, a.cols = cols, a.pitch = pitch, a.dy_stride = dy_stride, a.y_stride = dh_stride;
-  const bool vec = act8_vec(dy, dtype, cols, dy_stride, rows) && act8_vec(dh, dtype, cols, dh_stride, rows);
-  return act8_launch<kActGeluBack>(a, dtype, fmt, vec, static_cast<hipStream_t>(stream), what);
+  return act8_launch<kActGeluBack>(a, dtype, fmt, static_cast<hipStream_t>(stream), what);
 }
