@@ -189,12 +189,14 @@ def _input_grad(grad: torch.Tensor, weight: torch.Tensor, dtype: torch.dtype) ->
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, fmt):
+    def forward(ctx, x, weight, bias, fmt, kept):
         x_lp, w, b = (_cast(t, x.device.type) for t in (x, weight, bias))
         with torch.autocast(device_type=x.device.type, enabled=False):
             y = F.linear(x_lp, w, b)
         needs = ctx.needs_input_grad
-        ctx.kept = encode(x_lp, fmt) if needs[1] or needs[2] else None
+        if kept is None and (needs[1] or needs[2]):
+            kept = encode(x_lp, fmt)
+        ctx.kept = kept
         ctx.save_for_backward(w)
         ctx.dtypes = x.dtype, weight.dtype, None if bias is None else bias.dtype
         return y
@@ -211,15 +213,20 @@ class _Linear(torch.autograd.Function):
             dw, db = linear_backward(grad, ctx.kept, w_dtype, bias=needs[2])
             if db is not None and b_dtype != w_dtype:
                 db = db.to(b_dtype)
-        return dx, dw if needs[1] else None, db, None
+        return dx, dw if needs[1] else None, db, None, None
 
 
-def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
-           fmt: str = "int8") -> torch.Tensor:
-    """F.linear whose input is kept in 8 bits for the weight gradient."""
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, fmt: str = "int8",
+           kept: Optional[Act8] = None) -> torch.Tensor:
+    """F.linear whose input is kept in 8 bits for the weight gradient: as
+    `kept`, ``encode(x)`` made once for several layers of one input, or else
+    here in `fmt`."""
     need_float(x, "act8.linear")
-    _fmt(fmt, "act8.linear")
-    return _Linear.apply(x, weight, bias, fmt)
+    if kept is None:
+        _fmt(fmt, "act8.linear")
+    elif _kept(kept, "act8.linear").shape != x.shape:
+        raise ValueError(f"act8.linear: kept {tuple(kept.shape)} of an input {tuple(x.shape)}")
+    return _Linear.apply(x, weight, bias, fmt, kept)
 
 
 class _Gelu(torch.autograd.Function):
@@ -295,13 +302,14 @@ class CheckpointedLinears:
 def checkpoint_linears(model: nn.Module, module_filter: Optional[Callable[[str, nn.Module], bool]] = None,
                        fmt: str = "int8") -> CheckpointedLinears:
     """Puts every plain ``nn.Linear`` of `model` that `module_filter` selects
-    (all of them by default) on ``linear``.  Hooks on the modules run as before;
-    a module whose forward is replaced already is left as it is."""
+    (all of them by default) on ``linear``; their forwards take ``linear``'s
+    `kept` too, for layers that share an input.  Hooks on the modules run as
+    before; a module whose forward is replaced already is left as it is."""
     _fmt(fmt, "act8.checkpoint_linears")
 
-    def forward(module: nn.Linear, x: torch.Tensor) -> torch.Tensor:
-        if torch.is_grad_enabled() and x.device.type == "cuda":
-            return linear(x, module.weight, module.bias, fmt)
+    def forward(module: nn.Linear, x: torch.Tensor, kept: Optional[Act8] = None) -> torch.Tensor:
+        if torch.is_grad_enabled() and x.is_cuda:
+            return linear(x, module.weight, module.bias, fmt, kept)
         return F.linear(x, module.weight, module.bias)
 
     chosen = {}
