@@ -5,6 +5,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -55,3 +56,14 @@ def launch(name: str, device: torch.device, *args) -> None:
             rc = fn(*args, _native.stream_of(device))
     if rc != 0:
         _native._check(rc, name)
+
+
+def once(backward):
+    """A Function's backward that cannot be differentiated: torch's
+    once_differentiable where a graph of the backward is being made
+    (create_graph), the function itself, without that wrapper's cost, else."""
+    wrapped = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return wrapped(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return call

@@ -33,10 +33,9 @@ from typing import Callable, Optional, Tuple
 import torch
 import torch.nn.functional as F
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import _native
-from ._tensors import launch, need_float, rows2d, same_device
+from ._tensors import launch, need_float, once, rows2d, same_device
 
 __all__ = ["Act8", "FORMATS", "checkpoint_linears", "decode", "encode", "gelu", "gelu_backward", "gelu_forward",
            "linear", "linear_backward", "mlp"]
@@ -202,7 +201,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad):
         w, = ctx.saved_tensors
         x_dtype, w_dtype, b_dtype = ctx.dtypes
@@ -236,7 +235,7 @@ class _Gelu(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad):
         return gelu_backward(grad, ctx.kept), None
 
@@ -260,7 +259,7 @@ class _Mlp(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad):
         w1, w2 = ctx.saved_tensors
         needs, types_ = ctx.needs_input_grad, ctx.dtypes

@@ -11,10 +11,9 @@ import struct
 from typing import Optional, Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
-from ._tensors import launch, need_float, same_device, unit_last
+from ._tensors import launch, need_float, once, same_device, unit_last
 
 __all__ = ["qk_norm_rotary", "rotary_tables"]
 
@@ -23,7 +22,7 @@ STYLES = {"half": 0, "interleaved": 1}
 # smx_qk_desc, field by field: two sides, then the rest.
 _PACK = struct.Struct("5Q10q2i" * 2 + "3Q8qd2i")
 assert _PACK.size == _native.ctypes.sizeof(_native.QkDesc)
-_NO_STRIDES = (0, 0, 0)
+_NO_SIDE = (0,) * 17
 
 
 def rotary_tables(positions: int, rot: int, base: float = 10000.0,
@@ -35,62 +34,71 @@ def rotary_tables(positions: int, rot: int, base: float = 10000.0,
     return angle.cos().float(), angle.sin().float()
 
 
-def _side(x, w, dy, y, dw):
-    if x is None:
-        return (0,) * 17
+def _geometry(x, y):
+    """heads and the strides of x and y, as a side's descriptor holds them."""
+    return (x.shape[2], *x.stride()[:3], *y.stride()[:3])
+
+
+def _side(x, w, geometry, y, dy=None, dw=None):
+    ds = (0, 0, 0) if dy is None else dy.stride()[:3]
     return (x.data_ptr(), 0 if w is None else w.data_ptr(), 0 if dy is None else dy.data_ptr(), y.data_ptr(),
-            0 if dw is None else dw.data_ptr(), x.shape[2], *x.stride()[:3], *y.stride()[:3],
-            *(_NO_STRIDES if dy is None else dy.stride()[:3]), 0 if w is None else _native.dtype_code(w.dtype), 0)
+            0 if dw is None else dw.data_ptr(), *geometry, *ds, 0 if w is None else _native.dtype_code(w.dtype), 0)
 
 
-def _desc(q_side, k_side, x, cos, sin, positions, position0, eps, style):
+def _desc(q_side, k_side, x, cos, sin, positions, rest):
+    position0, eps, style = rest
     b, t, _, d = x.shape
     pos = (0, 0, 0) if positions is None else (positions.data_ptr(), *positions.stride())
-    packed = bytearray(_PACK.pack(*q_side, *k_side, cos.data_ptr(), sin.data_ptr(), *pos, position0, cos.shape[0], b, t,
-                                  d, 2 * cos.shape[1], eps, _native.dtype_code(x.dtype), style))
-    return _native.QkDesc.from_buffer(packed)
+    return _native.QkDesc.from_buffer(bytearray(_PACK.pack(
+        *q_side, *k_side, cos.data_ptr(), sin.data_ptr(), *pos, position0, cos.shape[0], b, t, d, 2 * cos.shape[1], eps,
+        _native.dtype_code(x.dtype), style)))
 
 
-def _forward(q, k, qw, kw, cos, sin, positions, position0, eps, style, out):
+def _forward(q, k, qw, kw, cos, sin, positions, rest, out=None):
+    """((q', k'), the sides' geometries)"""
     if out is None:
         out = (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device))
-    desc = _desc(_side(q, qw, None, out[0], None), _side(k, kw, None, out[1], None), q, cos, sin, positions, position0,
-                 eps, style)
-    launch("smx_qk_norm_rotary", q.device, desc)
-    return out
+    geometries = _geometry(q, out[0]), _geometry(k, out[1])
+    launch("smx_qk_norm_rotary", q.device, _desc(_side(q, qw, geometries[0], out[0]), _side(k, kw, geometries[1], out[1]),
+                                                 q, cos, sin, positions, rest))
+    return out, geometries
 
 
 class _QkNormRotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, qw, kw, cos, sin, positions, position0, eps, style):
+    def forward(ctx, q, k, qw, kw, cos, sin, positions, rest):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(q, k, qw, kw, cos, sin, positions)
-        ctx.rest = position0, eps, style
-        return _forward(q, k, qw, kw, cos, sin, positions, position0, eps, style, None)
+        out, ctx.geometries = _forward(q, k, qw, kw, cos, sin, positions, rest)
+        ctx.rest = rest
+        return out
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dq_out, dk_out):
         q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
-        position0, eps, style = ctx.rest
-        needs = ctx.needs_input_grad
-        sides, grads = [], []
-        for x, w, dy, need_x, need_w in ((q, qw, dq_out, needs[0], needs[2]), (k, kw, dk_out, needs[1], needs[3])):
-            if dy is None or not (need_x or need_w):
-                sides.append(_side(None, None, None, None, None))
-                grads.append((None, None))
-                continue
-            dy = unit_last(dy if dy.dtype == x.dtype else dy.to(x.dtype))
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            dw = torch.empty_like(w) if need_w else None
-            sides.append(_side(x, w, dy, dx, dw))
-            grads.append((dx if need_x else None, dw, dy))
-        if any(s[5] for s in sides):
-            need = _native.lib().smx_qk_workspace_bytes(q.shape[3]) if needs[2] or needs[3] else 0
-            work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-            desc = _desc(*sides, q, cos, sin, positions, position0, eps, style)
-            launch("smx_qk_norm_rotary_backward", q.device, desc, _native.ptr(work), need)
-        return grads[0][0], grads[1][0], grads[0][1], grads[1][1], None, None, None, None, None, None
+        need_q, need_k, need_qw, need_kw = ctx.needs_input_grad[:4]
+        # (dx is contiguous, as the result was: its strides are those of y)
+        q_side, dq, dqw = _side_backward(q, qw, dq_out, ctx.geometries[0], need_q, need_qw)
+        k_side, dk, dkw = _side_backward(k, kw, dk_out, ctx.geometries[1], need_k, need_kw)
+        if q_side is not _NO_SIDE or k_side is not _NO_SIDE:
+            work, need = None, 0
+            if need_qw or need_kw:
+                need = _native.lib().smx_qk_workspace_bytes(q.shape[3])
+                work = torch.empty(need, dtype=torch.uint8, device=q.device)
+            launch("smx_qk_norm_rotary_backward", q.device, _desc(q_side, k_side, q, cos, sin, positions, ctx.rest),
+                   None if work is None else work.data_ptr(), need)
+        return dq if need_q else None, dk if need_k else None, dqw, dkw, None, None, None, None
+
+
+def _side_backward(x, w, dy, geometry, need_x, need_w):
+    """(descriptor side, dx, dw) of one of the two, _NO_SIDE without a cotangent."""
+    if dy is None or not (need_x or need_w):
+        return _NO_SIDE, None, None
+    dy = unit_last(dy if dy.dtype == x.dtype else dy.to(x.dtype))
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = torch.empty_like(w) if need_w else None
+    return _side(x, w, geometry, dx, dy, dw), dx, dw
 
 
 def _weight(w, x, name):
@@ -142,7 +150,10 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
         positions, position0 = None, int(positions)
     same_device(what, q, k, q_weight, k_weight, cos, sin, positions)
     cos, sin = cos.contiguous(), sin.contiguous()
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+    rest = position0, float(eps), code
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
+                                        (q_weight is not None and q_weight.requires_grad) or
+                                        (k_weight is not None and k_weight.requires_grad))
     if out is not None:
         if grad:
             raise ValueError(f"{what}: out= is not supported under autograd")
@@ -152,5 +163,5 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
                                  "stride must be one")
     q, k = unit_last(q), unit_last(k)
     if grad:
-        return _QkNormRotary.apply(q, k, q_weight, k_weight, cos, sin, positions, position0, float(eps), code)
-    return _forward(q, k, q_weight, k_weight, cos, sin, positions, position0, float(eps), code, out)
+        return _QkNormRotary.apply(q, k, q_weight, k_weight, cos, sin, positions, rest)
+    return _forward(q, k, q_weight, k_weight, cos, sin, positions, rest, out)[0]

@@ -13,10 +13,9 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
-from ._tensors import launch, need_float, same_device, unit_last
+from ._tensors import launch, need_float, once, same_device, unit_last
 
 __all__ = ["policy_loss", "preference_loss", "token_logprobs"]
 
@@ -77,7 +76,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return lp
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad):
         logits, targets, mask, stats = ctx.saved_tensors
         return _logprobs_backward(logits, targets, mask, stats, grad.float(), grad.stride(), None), None, None
@@ -110,7 +109,7 @@ class _PolicyLoss(torch.autograd.Function):
         return loss, lp
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad_loss, _):
         grad, ctx.grad = ctx.grad, None
         if grad is None:
@@ -178,7 +177,7 @@ class _PreferenceLoss(torch.autograd.Function):
         return loss, margins
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad_loss, _):
         logits, targets, mask, stats, coef = ctx.saved_tensors
         return (_logprobs_backward(logits, targets, mask, stats, coef, (1, 0), grad_loss.float()),) + (None,) * 5
