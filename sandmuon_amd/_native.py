@@ -202,6 +202,26 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_ops = None
+
+
+def torch_ops():
+    """The torch bindings of the differentiable operators
+    (csrc/torch_ops.cpp), built beside the library."""
+    global _ops
+    if _ops is None:
+        lib()
+        try:
+            from . import _torch_ops
+        except ImportError as e:
+            raise ImportError(f"sandmuon_amd/_torch_ops.so does not load ({e}): build it with "
+                              "`python -m sandmuon_amd.build`. sandmuon_amd has no fallback path.") from e
+        if _torch_ops.abi_version != ABI_VERSION:
+            raise ImportError(f"_torch_ops.so has ABI {_torch_ops.abi_version}, expected {ABI_VERSION}; rebuild it")
+        _ops = _torch_ops
+    return _ops
+
+
 def _check(rc: int, what: str) -> None:
     if rc != 0:
         msg = lib().smx_last_error().decode(errors="replace")
