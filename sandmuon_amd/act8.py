@@ -33,9 +33,9 @@ from typing import Callable, Optional, Tuple
 import torch
 import torch.nn.functional as F
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import _native
-from ._tensors import launch, need_float, once, rows2d, same_device
 
 __all__ = ["Act8", "FORMATS", "checkpoint_linears", "decode", "encode", "gelu", "gelu_backward", "gelu_forward",
            "linear", "linear_backward", "mlp"]
@@ -55,15 +55,22 @@ class Act8:
     """A kept activation: codes [rows, pitch] and scale bytes [rows, pitch /
     32] in one buffer, with the activation's shape and format."""
 
-    __slots__ = ("data", "shape", "rows", "cols", "pitch", "fmt")
+    __slots__ = ("data", "shape", "fmt")
 
-    def __init__(self, shape: torch.Size, fmt: str, device):
-        self.shape = shape
-        self.cols = shape[-1]
-        self.rows = rows = shape[0] if len(shape) == 2 else shape[:-1].numel()
-        self.pitch = pitch = -(-shape[-1] // _BLOCK) * _BLOCK
-        self.fmt = fmt
-        self.data = torch.empty(rows * (pitch + pitch // _BLOCK), dtype=torch.uint8, device=device)
+    def __init__(self, data: torch.Tensor, shape: torch.Size, fmt: str):
+        self.data, self.shape, self.fmt = data, shape, fmt
+
+    @property
+    def rows(self) -> int:
+        return self.shape[:-1].numel()
+
+    @property
+    def cols(self) -> int:
+        return self.shape[-1]
+
+    @property
+    def pitch(self) -> int:
+        return -(-self.shape[-1] // _BLOCK) * _BLOCK
 
     @property
     def codes(self) -> torch.Tensor:
@@ -77,17 +84,6 @@ class Act8:
     def nbytes(self) -> int:
         return self.data.numel()
 
-    def _ptrs(self) -> Tuple[int, int]:
-        at = self.data.data_ptr()
-        return at, at + self.rows * self.pitch
-
-
-def _activation(x: torch.Tensor, what: str) -> torch.Tensor:
-    need_float(x, what)
-    if x.dim() < 1:
-        raise ValueError(f"{what}: expected at least one dimension")
-    return x.detach() if x.requires_grad else x
-
 
 def _kept(saved: Act8, what: str) -> Act8:
     if not isinstance(saved, Act8):
@@ -97,54 +93,26 @@ def _kept(saved: Act8, what: str) -> Act8:
 
 def encode(x: torch.Tensor, fmt: str = "int8") -> Act8:
     """x [..., d] (float32, bfloat16 or float16) in 8 bits."""
-    code = _fmt(fmt, "act8.encode")
-    x = _activation(x, "act8.encode")
-    rows = rows2d(x)
-    saved = Act8(x.shape, fmt, x.device)
-    codes, scales = saved._ptrs()
-    launch("smx_act8_encode", rows.device, rows.data_ptr(), _native.dtype_code(rows.dtype), saved.rows, saved.cols,
-           rows.stride(0), code, codes, scales, saved.pitch)
-    return saved
+    return Act8(_native.torch_ops().act8_encode(x, _fmt(fmt, "act8.encode")), x.shape, fmt)
 
 
 def decode(saved: Act8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The kept values in `dtype`: exact in bfloat16 and float32."""
     _kept(saved, "act8.decode")
-    out = torch.empty(saved.shape, dtype=dtype, device=saved.data.device)
-    codes, scales = saved._ptrs()
-    launch("smx_act8_decode", out.device, codes, scales, FORMATS[saved.fmt], saved.rows, saved.cols, saved.pitch,
-           out.data_ptr(), _native.dtype_code(dtype), saved.cols)
-    return out
+    return _native.torch_ops().act8_decode(saved.data, saved.shape, FORMATS[saved.fmt], dtype)
 
 
 def gelu_forward(h: torch.Tensor, fmt: str = "int8",
                  keep_output: bool = True) -> Tuple[torch.Tensor, Act8, Optional[Act8]]:
     """(GELU(h), h kept, the GELU's output kept or None) in one pass."""
-    code = _fmt(fmt, "act8.gelu_forward")
-    h = _activation(h, "act8.gelu_forward")
-    rows = rows2d(h)
-    y = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-    kept_h = Act8(h.shape, fmt, h.device)
-    kept_y = Act8(h.shape, fmt, h.device) if keep_output else None
-    launch("smx_act8_gelu", rows.device, rows.data_ptr(), _native.dtype_code(h.dtype), kept_h.rows, kept_h.cols,
-           rows.stride(0), code, y.data_ptr(), kept_h.cols, *kept_h._ptrs(), *(kept_y._ptrs() if keep_output else
-           (None, None)), kept_h.pitch)
-    return y, kept_h, kept_y
+    y, kept_h, kept_y = _native.torch_ops().act8_gelu(h, _fmt(fmt, "act8.gelu_forward"), keep_output)
+    return y, Act8(kept_h, h.shape, fmt), Act8(kept_y, h.shape, fmt) if keep_output else None
 
 
 def gelu_backward(dy: torch.Tensor, saved: Act8) -> torch.Tensor:
     """dy * GELU'(kept h), in dy's type."""
     _kept(saved, "act8.gelu_backward")
-    dy = _activation(dy, "act8.gelu_backward")
-    if dy.shape != saved.shape:
-        raise ValueError(f"act8.gelu_backward: cotangent {tuple(dy.shape)} of a kept {tuple(saved.shape)}")
-    same_device("act8.gelu_backward", dy, saved.data)
-    rows = rows2d(dy)
-    dh = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-    codes, scales = saved._ptrs()
-    launch("smx_act8_gelu_backward", rows.device, rows.data_ptr(), _native.dtype_code(dy.dtype), saved.rows,
-           saved.cols, rows.stride(0), codes, scales, FORMATS[saved.fmt], saved.pitch, dh.data_ptr(), saved.cols)
-    return dh
+    return _native.torch_ops().act8_gelu_backward(dy, saved.data, saved.shape, FORMATS[saved.fmt])
 
 
 def linear_backward(delta: torch.Tensor, saved: Act8, dtype: Optional[torch.dtype] = None,
@@ -153,24 +121,7 @@ def linear_backward(delta: torch.Tensor, saved: Act8, dtype: Optional[torch.dtyp
     [..., n] and kept input `saved` [..., d], in `dtype` (delta's by default),
     each rounded once from FP32 sums."""
     _kept(saved, "act8.linear_backward")
-    delta = _activation(delta, "act8.linear_backward")
-    if delta.shape[:-1] != saved.shape[:-1]:
-        raise ValueError(f"act8.linear_backward: cotangent {tuple(delta.shape)} of a kept input {tuple(saved.shape)}")
-    same_device("act8.linear_backward", delta, saved.data)
-    rows = rows2d(delta)
-    n = delta.shape[-1]
-    dtype = delta.dtype if dtype is None else dtype
-    out = _native.dtype_code(dtype)
-    code = _native.dtype_code(delta.dtype)
-    lib = _native.lib()
-    dw = torch.empty(n, saved.cols, dtype=dtype, device=delta.device)
-    db = torch.empty(n, dtype=dtype, device=delta.device) if bias else None
-    need = lib.smx_act8_wgrad_workspace_bytes(saved.rows, n, saved.cols, code)
-    work = torch.empty(need, dtype=torch.uint8, device=delta.device) if need else None
-    codes, scales = saved._ptrs()
-    launch("smx_act8_wgrad", rows.device, rows.data_ptr(), code, saved.rows, n, rows.stride(0), codes, scales,
-           FORMATS[saved.fmt], saved.cols, saved.pitch, dw.data_ptr(), _native.ptr(db), out, _native.ptr(work), need)
-    return dw, db
+    return _native.torch_ops().act8_linear_backward(delta, saved.data, saved.shape, FORMATS[saved.fmt], dtype, bias)
 
 
 # ------------------------------------------------- differentiable functions ---
@@ -201,7 +152,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once
+    @once_differentiable
     def backward(ctx, grad):
         w, = ctx.saved_tensors
         x_dtype, w_dtype, b_dtype = ctx.dtypes
@@ -220,7 +171,6 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     """F.linear whose input is kept in 8 bits for the weight gradient: as
     `kept`, ``encode(x)`` made once for several layers of one input, or else
     here in `fmt`."""
-    need_float(x, "act8.linear")
     if kept is None:
         _fmt(fmt, "act8.linear")
     elif _kept(kept, "act8.linear").shape != x.shape:
@@ -235,7 +185,7 @@ class _Gelu(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once
+    @once_differentiable
     def backward(ctx, grad):
         return gelu_backward(grad, ctx.kept), None
 
@@ -243,7 +193,7 @@ class _Gelu(torch.autograd.Function):
 def gelu(h: torch.Tensor, fmt: str = "int8") -> torch.Tensor:
     """F.gelu (exact form) whose input is kept in 8 bits."""
     _fmt(fmt, "act8.gelu")
-    return _Gelu.apply(need_float(h, "act8.gelu"), fmt)
+    return _Gelu.apply(h, fmt)
 
 
 class _Mlp(torch.autograd.Function):
@@ -259,7 +209,7 @@ class _Mlp(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once
+    @once_differentiable
     def backward(ctx, grad):
         w1, w2 = ctx.saved_tensors
         needs, types_ = ctx.needs_input_grad, ctx.dtypes
@@ -281,7 +231,6 @@ def mlp(x: torch.Tensor, fc_weight: torch.Tensor, fc_bias: Optional[torch.Tensor
         proj_bias: Optional[torch.Tensor], fmt: str = "int8") -> torch.Tensor:
     """proj(GELU(fc(x))) with x, the hidden layer and the GELU's output kept in
     8 bits: 1 byte an element where three 16-bit tensors would be kept."""
-    need_float(x, "act8.mlp")
     _fmt(fmt, "act8.mlp")
     return _Mlp.apply(x, fc_weight, fc_bias, proj_weight, proj_bias, fmt)
 

@@ -411,6 +411,124 @@ std::tuple<Tensor, Tensor> preference_loss(Tensor logits, Tensor targets, OptTen
   return {y[0], y[1]};
 }
 
+// ----------------------------------------------------------------- act8 ---
+// A kept activation: codes [rows, pitch], then scale bytes [rows, pitch / 32].
+struct Kept {
+  Tensor data;
+  int64_t rows, cols, pitch;
+  // A new one for an activation like `x`.
+  static Kept for_rows(const Tensor &x, int64_t rows, int64_t cols) {
+    const int64_t pitch = (cols + 31) / 32 * 32;
+    return {at::empty({rows * (pitch + pitch / 32)}, x.options().dtype(torch::kUInt8)), rows, cols, pitch};
+  }
+  // The one in `data`, of an activation of this shape.
+  static Kept in(const Tensor &data, at::IntArrayRef shape) {
+    TORCH_CHECK_VALUE(!shape.empty(), "a kept activation has at least one dimension");
+    const int64_t rows = c10::multiply_integers(shape.slice(0, shape.size() - 1)), cols = shape.back();
+    const int64_t pitch = (cols + 31) / 32 * 32;
+    TORCH_CHECK_VALUE(data.is_cuda() && data.scalar_type() == torch::kUInt8 && data.is_contiguous() &&
+                          data.numel() == rows * (pitch + pitch / 32),
+                      "the bytes of a kept ", shape, ": ", data.sizes(), " ", data.scalar_type(), " on ", data.device());
+    return {data, rows, cols, pitch};
+  }
+  uint8_t *codes() const { return data.data_ptr<uint8_t>(); }
+  uint8_t *scales() const { return codes() + rows * pitch; }
+};
+
+// x as [rows, cols] with unit column stride (a copy where its strides allow no such view).
+Tensor rows2d(const Tensor &x, const char *what) {
+  need_float(x, what);
+  TORCH_CHECK_VALUE(x.dim() >= 1, what, ": expected at least one dimension");
+  const Tensor t = x.requires_grad() ? x.detach() : x;
+  if (t.dim() == 2) return unit_last(t);
+  const int64_t cols = t.size(-1);
+  return unit_last(t.reshape({cols ? t.numel() / cols : c10::multiply_integers(t.sizes().slice(0, t.dim() - 1)), cols}));
+}
+
+int out_dtype(torch::ScalarType type) {
+  switch (type) {
+    case torch::kFloat32: return SMX_F32;
+    case torch::kBFloat16: return SMX_BF16;
+    case torch::kFloat16: return SMX_F16;
+    default: TORCH_CHECK_VALUE(false, "unsupported dtype ", type, "; expected float32, bfloat16 or float16");
+  }
+}
+
+Tensor act8_encode(const Tensor &x, int64_t fmt) {
+  const Tensor r = rows2d(x, "act8.encode");
+  const Kept k = Kept::for_rows(r, r.size(0), r.size(1));
+  const c10::DeviceGuard guard(r.device());
+  check(smx_act8_encode(r.data_ptr(), dtype_of(r), k.rows, k.cols, r.stride(0), static_cast<int>(fmt), k.codes(),
+                        k.scales(), k.pitch, stream_of(r)),
+        "smx_act8_encode");
+  return k.data;
+}
+
+Tensor act8_decode(const Tensor &data, at::IntArrayRef shape, int64_t fmt, torch::ScalarType type) {
+  const int code = out_dtype(type);
+  const Kept k = Kept::in(data, shape);
+  const Tensor out = at::empty(shape, data.options().dtype(type));
+  const c10::DeviceGuard guard(data.device());
+  check(smx_act8_decode(k.codes(), k.scales(), static_cast<int>(fmt), k.rows, k.cols, k.pitch, out.data_ptr(), code, k.cols,
+                        stream_of(data)),
+        "smx_act8_decode");
+  return out;
+}
+
+std::tuple<Tensor, Tensor, OptTensor> act8_gelu(const Tensor &h, int64_t fmt, bool keep_output) {
+  const Tensor r = rows2d(h, "act8.gelu_forward");
+  const Tensor y = at::empty(h.sizes(), r.options());
+  const Kept kh = Kept::for_rows(r, r.size(0), r.size(1));
+  std::optional<Kept> ky;
+  if (keep_output) ky = Kept::for_rows(r, kh.rows, kh.cols);
+  const c10::DeviceGuard guard(r.device());
+  check(smx_act8_gelu(r.data_ptr(), dtype_of(r), kh.rows, kh.cols, r.stride(0), static_cast<int>(fmt), y.data_ptr(), kh.cols,
+                      kh.codes(), kh.scales(), ky ? ky->codes() : nullptr, ky ? ky->scales() : nullptr, kh.pitch,
+                      stream_of(r)),
+        "smx_act8_gelu");
+  return {y, kh.data, ky ? OptTensor(ky->data) : std::nullopt};
+}
+
+Tensor act8_gelu_backward(const Tensor &dy, const Tensor &data, at::IntArrayRef shape, int64_t fmt) {
+  const char *what = "act8.gelu_backward";
+  const Tensor r = rows2d(dy, what);
+  TORCH_CHECK_VALUE(dy.sizes() == shape, what, ": cotangent ", dy.sizes(), " of a kept ", shape);
+  const OptTensor d = data;
+  same_device(what, dy, {&d});
+  const Kept k = Kept::in(data, shape);
+  const Tensor dh = at::empty(dy.sizes(), r.options());
+  const c10::DeviceGuard guard(r.device());
+  check(smx_act8_gelu_backward(r.data_ptr(), dtype_of(r), k.rows, k.cols, r.stride(0), k.codes(), k.scales(),
+                               static_cast<int>(fmt), k.pitch, dh.data_ptr(), k.cols, stream_of(r)),
+        "smx_act8_gelu_backward");
+  return dh;
+}
+
+std::tuple<Tensor, OptTensor> act8_linear_backward(const Tensor &delta, const Tensor &data, at::IntArrayRef shape,
+                                                   int64_t fmt, std::optional<torch::ScalarType> type, bool bias) {
+  const char *what = "act8.linear_backward";
+  const Tensor r = rows2d(delta, what);
+  TORCH_CHECK_VALUE(delta.dim() == static_cast<int64_t>(shape.size()) &&
+                        delta.sizes().slice(0, delta.dim() - 1) == shape.slice(0, shape.size() - 1),
+                    what, ": cotangent ", delta.sizes(), " of a kept input ", shape);
+  const OptTensor d = data;
+  same_device(what, delta, {&d});
+  const auto out = r.options().dtype(type.value_or(r.scalar_type()));
+  const int code = out_dtype(type.value_or(r.scalar_type()));
+  const Kept k = Kept::in(data, shape);
+  const int64_t n = r.size(1);
+  const Tensor dw = at::empty({n, k.cols}, out);
+  OptTensor db;
+  if (bias) db = at::empty({n}, out);
+  const int64_t bytes = smx_act8_wgrad_workspace_bytes(k.rows, n, k.cols, dtype_of(r));
+  const Tensor work = at::empty({bytes}, r.options().dtype(torch::kUInt8));
+  const c10::DeviceGuard guard(r.device());
+  check(smx_act8_wgrad(r.data_ptr(), dtype_of(r), k.rows, n, r.stride(0), k.codes(), k.scales(), static_cast<int>(fmt),
+                       k.cols, k.pitch, dw.data_ptr(), ptr(db), code, work.data_ptr(), bytes, stream_of(r)),
+        "smx_act8_wgrad");
+  return {dw, db};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -419,4 +537,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("token_logprobs", &token_logprobs);
   m.def("policy_loss", &policy_loss);
   m.def("preference_loss", &preference_loss);
+  m.def("act8_encode", &act8_encode);
+  m.def("act8_decode", &act8_decode);
+  m.def("act8_gelu", &act8_gelu);
+  m.def("act8_gelu_backward", &act8_gelu_backward);
+  m.def("act8_linear_backward", &act8_linear_backward);
 }
