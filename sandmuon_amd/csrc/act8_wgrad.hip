@@ -136,6 +136,38 @@ __device__ __forceinline__ int lds_at(int row, int block) {
   return row * 2 * T + ((block ^ ((row & 3) << 1)) << 5);
 }
 
+// The first n of four neighbours of dw, at their own alignment.
+__device__ __forceinline__ void store_row4(void *dw, int out, int64_t i, const float4 &v, int64_t n) {
+  const float e[4] = {v.x, v.y, v.z, v.w};
+  if (out == SMX_F32) {
+    typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+    float *p = static_cast<float *>(dw) + i;
+    if (n >= 4) {
+      *reinterpret_cast<v4 *>(p) = v4{v.x, v.y, v.z, v.w};
+    } else {
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        if (q < n) p[q] = e[q];
+    }
+  } else {
+    uint16_t h[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const _Float16 half = static_cast<_Float16>(e[q]);
+      h[q] = out == SMX_BF16 ? f32_to_bf16_bits(e[q]) : __builtin_bit_cast(uint16_t, half);
+    }
+    typedef uint32_t v2 __attribute__((ext_vector_type(2), aligned(2)));
+    uint16_t *p = static_cast<uint16_t *>(dw) + i;
+    if (n >= 4) {
+      *reinterpret_cast<v2 *>(p) = v2{h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16};
+    } else {
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        if (q < n) p[q] = h[q];
+    }
+  }
+}
+
 template <int DT, int FMT, class C>
 __global__ void __launch_bounds__(C::kThreads, C::kWavesPerSimd) wgrad_kernel(WgradArgs a) {
   constexpr int P = parts_of(DT), kStep = C::step(DT), TN = C::kTileN, TK = C::kTileK;
@@ -144,7 +176,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kWavesPerSimd) wgrad_kernel(Wg
   constexpr int kDeltaLoads = kStep / kDeltaRows, kCodeLoads = kStep / kCodeRows;
   static_assert(kDeltaLoads * kDeltaRows == kStep && kCodeLoads * kCodeRows == kStep, "whole passes");
   constexpr int FN = TN / C::kWavesN / 32, FK = TK / C::kWavesK / 32;  // a wave's MFMA tiles
-  __shared__ __attribute__((aligned(128))) char lds[2 * kBuffer];
+  // dw's tile leaves through LDS too, in passes of a row of waves each where it is wide
+  constexpr int kPasses = TN * TK * 4 > 65536 ? C::kWavesN : 1, kPassRows = TN / kPasses;
+  __shared__ __attribute__((aligned(128))) char lds[kPassRows * TK * 4 > 2 * kBuffer ? kPassRows * TK * 4 : 2 * kBuffer];
 
   // Blocks of one split run on one XCD as far as they can, since they share its rows.
   const int64_t blocks = static_cast<int64_t>(a.tiles) * a.splits;
@@ -307,37 +341,37 @@ __global__ void __launch_bounds__(C::kThreads, C::kWavesPerSimd) wgrad_kernel(Wg
     __syncthreads();
   }
 
-  // Lane l holds column l mod 32 and rows 8 (r / 4) + 4 (l / 32) + r mod 4: an
-  // offset of the lane's own, from addresses that the wave shares.
-  const auto each = [&](auto store) __attribute__((always_inline)) {
-    const int64_t nb = n0 + wn, kb = k0 + wk;
-    const int ln = 4 * (lane >> 5), lk = lane & 31;
-    const uint32_t off = static_cast<uint32_t>(ln) * static_cast<uint32_t>(a.k) + lk;
-    const bool inside = nb + 32 * FN <= a.n && kb + 32 * FK <= a.k;
-    int64_t at = (a.splits > 1 ? static_cast<int64_t>(split) * a.n * a.k : 0) + nb * a.k + kb;
+  // The tile goes out through LDS, row by row: lane l of a wave holds column l
+  // mod 32 and rows 8 (r / 4) + 4 (l / 32) + r mod 4 of an MFMA tile.  (Stores
+  // from there, one element a lane, took five times the code, which the first
+  // blocks of a short launch wait for.)
+  float *tile_out = reinterpret_cast<float *>(lds);
+  const int64_t part = a.splits > 1 ? static_cast<int64_t>(split) * a.n * a.k : 0;
+#pragma unroll 1
+  for (int pass = 0; pass < kPasses; ++pass) {
+    if (kPasses == 1 || wn == pass * kPassRows) {
+      float *at = tile_out + (wn - pass * kPassRows + 4 * (lane >> 5)) * TK + wk + (lane & 31);
 #pragma unroll
-    for (int f = 0; f < FN; ++f)
+      for (int f = 0; f < FN; ++f)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = 32 * f + 8 * (r >> 2) + (r & 3);
+        for (int h = 0; h < FK; ++h)
 #pragma unroll
-        for (int h = 0; h < FK; ++h) {
-          float v = acc[f][h][r];
-          // (keeps the compiler from moving every sum and address at once)
-          asm volatile("" : "+s"(at), "+v"(v));
-          if (inside || (nb + row + ln < a.n && kb + 32 * h + lk < a.k)) store(at + 32 * h, off, v);
-        }
-        at += (r & 3) == 3 ? 5 * a.k : a.k;
-      }
-  };
-  if (a.out == SMX_F32) {
-    each([&](int64_t i, uint32_t o, float v) __attribute__((always_inline)) { (static_cast<float *>(a.dw) + i)[o] = v; });
-  } else {
-    each([&](int64_t i, uint32_t o, float v) __attribute__((always_inline)) {
-      const _Float16 half = static_cast<_Float16>(v);
-      (static_cast<uint16_t *>(a.dw) + i)[o] = a.out == SMX_BF16 ? f32_to_bf16_bits(v) : __builtin_bit_cast(uint16_t, half);
-    });
+          for (int r = 0; r < 16; ++r) at[(32 * f + 8 * (r >> 2) + (r & 3)) * TK + 32 * h] = acc[f][h][r];
+    }
+    __syncthreads();
+    constexpr int kPerRow = TK / 4, kAtOnce = C::kThreads / kPerRow;
+    const int col = 4 * (tid % kPerRow);
+    const int64_t k = k0 + col;
+    const int64_t rows_here = min<int64_t>(kPassRows, a.n - n0 - pass * kPassRows);
+#pragma unroll 4
+    for (int row = tid / kPerRow; row < rows_here; row += kAtOnce) {
+      const float4 v = *reinterpret_cast<const float4 *>(tile_out + row * TK + col);
+      const int64_t o = part + (n0 + pass * kPassRows + row) * a.k + k;
+      store_row4(a.dw, a.out, o, v, a.k - k);
+    }
+    if (kPasses > 1) __syncthreads();
   }
+  if (kPasses == 1) __syncthreads();
   if (a.db) {
     float *red = reinterpret_cast<float *>(lds);  // [rows of threads][TN]
 #pragma unroll
