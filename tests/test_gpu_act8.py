@@ -328,3 +328,64 @@ def test_refusals(device):
         act8.gelu_backward(x, x)
     with pytest.raises(ValueError, match="dimension"):
         act8.encode(torch.tensor(1.0, device=device))
+
+
+def test_side_stream_and_graph(device):
+    """On a stream of their own, and replayed from a graph, the same bits."""
+    from sandmuon_amd.attention import qk_norm_rotary, rotary_tables
+    x = activation(3000, 256, torch.bfloat16, device, 1)
+    delta = activation(3000, 192, torch.bfloat16, device, 2)
+    cos, sin = rotary_tables(64, 64, device=device)
+    w = torch.ones(64, device=device)
+
+    def step(x, delta):
+        saved = act8.encode(x)
+        y, kept, kept_y = act8.gelu_forward(x, "e4m3")
+        q = x[:2944].view(46, 64, 4, 64).detach().requires_grad_()
+        k = delta[:2944].view(46, 64, 3, 64).detach().requires_grad_()
+        out = qk_norm_rotary(q, k, w.requires_grad_(), None, cos, sin)
+        grads = torch.autograd.grad(out, (q, k, w), (out[1].detach().repeat(1, 1, 2, 1)[:, :, :4], out[0].detach()[:, :, :3]))
+        return (*act8.linear_backward(delta, saved, torch.float32), act8.decode(saved), y, act8.gelu_backward(y, kept),
+                act8.decode(kept_y), *(o.detach() for o in out), *grads)
+
+    want = step(x, delta)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(x, delta)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    held = x.clone()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(held, delta)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(held, delta)
+    for k in range(3):
+        held.copy_(x * (1 + 0.5 * k))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, step(held, delta)))
+
+
+def test_no_double_backward(device):
+    from sandmuon_amd import losses
+    from sandmuon_amd.attention import qk_norm_rotary, rotary_tables
+    z = torch.randn(2, 3, 40, device=device, requires_grad=True)
+    y = torch.zeros(2, 3, dtype=torch.long, device=device)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(losses.token_logprobs(z, y).sum(), z, create_graph=True)
+    q = torch.randn(1, 2, 1, 64, device=device, requires_grad=True)
+    out, _ = qk_norm_rotary(q, q.detach(), None, None, *rotary_tables(4, 64, device=device))
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(out.sum(), q, create_graph=True)
+
+
+def test_bytes_that_do_not_fit_their_shape_are_refused(device):
+    saved = act8.encode(torch.randn(8, 64, device=device))
+    for shape, data in ((torch.Size([9, 64]), saved.data), (torch.Size([8, 64]), saved.data[:-1]),
+                        (torch.Size([8, 64]), saved.data.float()), (torch.Size([8, 64]), saved.data.cpu())):
+        with pytest.raises(ValueError, match="bytes of a kept"):
+            act8.decode(act8.Act8(data, shape, "int8"))
