@@ -397,8 +397,10 @@ __global__ void __launch_bounds__(256) wgrad_join_kernel(const float *part, int6
     const int col = threadIdx.x & 15, q = threadIdx.x >> 4;
     const int64_t j = (blockIdx.x - dw_blocks) * 16 + col;
     float t = 0.f;
-    if (j < n)
+    if (j < n) {
+#pragma unroll 4
       for (int s = q; s < db_parts; s += 16) t += part_db[s * n + j];
+    }
     red[q][col] = t;
     __syncthreads();
     if (q > 0 || j >= n) return;
@@ -409,7 +411,16 @@ __global__ void __launch_bounds__(256) wgrad_join_kernel(const float *part, int6
   const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
   if (i0 + 4 <= count && count % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
     float4 t = make_float4(0, 0, 0, 0);
-    for (int s = 0; s < splits; ++s) {
+    int s = 0;
+    for (; s + 8 <= splits; s += 8) {  // (eight loads in flight, added in order)
+      float4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const float4 *>(part + (s + u) * count + i0);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) t.x += v[u].x, t.y += v[u].y, t.z += v[u].z, t.w += v[u].w;
+    }
+#pragma unroll 4
+    for (; s < splits; ++s) {
       const float4 v = *reinterpret_cast<const float4 *>(part + s * count + i0);
       t.x += v.x, t.y += v.y, t.z += v.z, t.w += v.w;
     }
