@@ -8,6 +8,11 @@
 // thread divides.  One row a thread: waves, not loads of a thread, hide the
 // latency (four rows a thread took 68 us for the GELU of 16384 x 3072 bf16
 // instead of 54, at half the waves).
+//
+// Measured at 16384 x 3072 bf16, int8: GELU with both sides kept 54 us (6 bytes
+// an element: 5.6 TB/s), its gradient 58 us (5 bytes: 4.4 TB/s, bound by its 27
+// vector instructions an element as much as by HBM), read back 24 us; 16384 x
+// 768 bf16 kept 8 us (4.7 TB/s).
 #include "act8.h"
 
 #include <algorithm>

@@ -10,10 +10,16 @@
 // with a BF16 cotangent is exact in FP32.  FP16 and FP32 cotangents are staged
 // as the two or three BF16 parts that sum to them exactly, with a product each.
 //
-// The two LDS buffers alternate: while one step's MFMAs run, the next step's
-// registers are written to the other and the loads of the step after are in
-// flight.  Splits of m write FP32 partial tiles that a second launch adds in
+// The two LDS buffers alternate: beside one step's MFMAs the next step is
+// written to the other, and loads of a later step are in flight.  Splits of m write FP32 partial tiles that a second launch adds in
 // order, so the result does not depend on timing.
+//
+// Measured, BF16 cotangents, with db: 8192 x 2048 -> 8192 253 us in e4m3 (1.09
+// PFLOP/s) and 287 us in int8, whose codes take 2.5 vector instructions an element
+// to widen where e4m3 takes half of one; 16384 x 768 -> 3072 92 and 97 us; 16384 x
+// 768 -> 768 (small tiles, 14 splits) 38 us, 7 of them the join.  The wide tile is
+// bound by MFMA issue and the clock held under it (MFMAs busy 41% of the cycles,
+// LDS 31%), the small one by staging (28%).
 #include "act8.h"
 
 #include <algorithm>
