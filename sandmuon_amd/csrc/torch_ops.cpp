@@ -65,6 +65,12 @@ bool integral(const Tensor &t) { return c10::isIntegralType(t.scalar_type(), fal
 // t, or a contiguous copy where its last dimension has no unit stride.
 Tensor unit_last(const Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
+// And where its rows overlap (the gradient of a sum over them is one row
+// repeated): the entry points take rows that lie behind each other.
+Tensor apart_rows(const Tensor &t) {
+  return t.size(-2) > 1 && t.stride(-2) < t.size(-1) ? t.contiguous() : unit_last(t);
+}
+
 template <typename T = void>
 T *ptr(const OptTensor &t) {
   return t.has_value() && t->defined() ? static_cast<T *>(t->data_ptr()) : nullptr;
@@ -239,7 +245,7 @@ void check_logits(const char *what, Tensor *logits, Tensor *targets, OptTensor *
   }
   const OptTensor t = *targets;
   same_device(what, *logits, {&t, mask});
-  *logits = unit_last(*logits);
+  *logits = apart_rows(*logits);
   *targets = targets->to(torch::kInt64).contiguous();
 }
 
@@ -440,9 +446,9 @@ Tensor rows2d(const Tensor &x, const char *what) {
   need_float(x, what);
   TORCH_CHECK_VALUE(x.dim() >= 1, what, ": expected at least one dimension");
   const Tensor t = x.requires_grad() ? x.detach() : x;
-  if (t.dim() == 2) return unit_last(t);
+  if (t.dim() == 2) return apart_rows(t);
   const int64_t cols = t.size(-1);
-  return unit_last(t.reshape({cols ? t.numel() / cols : c10::multiply_integers(t.sizes().slice(0, t.dim() - 1)), cols}));
+  return apart_rows(t.reshape({cols ? t.numel() / cols : c10::multiply_integers(t.sizes().slice(0, t.dim() - 1)), cols}));
 }
 
 int out_dtype(torch::ScalarType type) {

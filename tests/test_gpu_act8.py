@@ -389,3 +389,37 @@ def test_bytes_that_do_not_fit_their_shape_are_refused(device):
                         (torch.Size([8, 64]), saved.data.float()), (torch.Size([8, 64]), saved.data.cpu())):
         with pytest.raises(ValueError, match="bytes of a kept"):
             act8.decode(act8.Act8(data, shape, "int8"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_rows_that_overlap(device, dtype):
+    row = activation(1, 70, dtype, device, 21)
+    strip = activation(1, 300, dtype, device, 22)[0]
+    for x in (row.expand(9, 70), row.expand(3, 3, 70), strip.unfold(0, 70, 3), row[:, :1].expand(9, 70)):
+        plain = x.contiguous()
+        saved = act8.encode(x)
+        assert torch.equal(saved.data, act8.encode(plain).data)
+        y, kept, _ = act8.gelu_forward(x)
+        assert torch.equal(y, act8.gelu_forward(plain)[0]) and torch.equal(kept.data, saved.data)
+        assert torch.equal(act8.gelu_backward(x, saved), act8.gelu_backward(plain, saved))
+        for got, want in zip(act8.linear_backward(x, saved), act8.linear_backward(plain, saved)):
+            assert torch.equal(got, want)
+
+
+def test_gradients_of_sums_over_rows(device):
+    # the cotangent is one row, repeated
+    h = activation(33, 40, torch.float32, device, 23)
+    w = activation(24, 40, torch.float32, device, 24) / 8
+    for fn in (lambda x, v: act8.gelu(x), lambda x, v: act8.linear(x, v), lambda x, v: act8.mlp(x, v, None, v.t(), None)):
+        grads = []
+        for repeat in (False, True):
+            leaf, weight = h.clone().requires_grad_(), w.clone().requires_grad_()
+            y = fn(leaf, weight)
+            cot = torch.linspace(-1, 1, y.shape[-1], device=device)
+            if repeat:
+                y.sum(0).backward(cot)
+            else:
+                y.backward(cot.expand(33, -1).contiguous())
+            grads.append((leaf.grad, weight.grad))
+        for a, b in zip(*grads):
+            assert (a is None and b is None) or torch.equal(a, b)

@@ -356,3 +356,23 @@ def test_refusals(device):
         losses.preference_loss(logits[:1], targets[:1], ref[:1])
     with pytest.raises(ValueError, match="label_smoothing"):
         losses.preference_loss(logits, targets, ref, label_smoothing=1.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_rows_that_overlap(device, dtype):
+    one, targets, mask, old, ref, adv = make(device, 4, 6, 97, dtype, 30)
+    strip = make(device, 1, 1, 400, dtype, 31)[0][0, 0]
+    for view in (one[:, :1].expand(4, 6, 97), one[:1, :1].expand(4, 6, 97), strip.unfold(0, 97, 10)[:24].view(4, 6, 97),
+                 one[..., :1].expand(4, 6, 97)):
+        results = []
+        for z in (view, view.contiguous()):
+            z = z.detach().requires_grad_()
+            lp = losses.token_logprobs(z, targets, mask)
+            lp_grad, = torch.autograd.grad(lp.sum(), z)
+            loss, _ = losses.policy_loss(z, targets, adv, old_logprobs=old, ref_logprobs=ref, mask=mask, kl_coef=0.1)
+            policy, = torch.autograd.grad(loss, z)
+            loss2, margins = losses.preference_loss(z, targets, ref, mask=mask)
+            pref, = torch.autograd.grad(loss2, z)
+            results.append((lp.detach(), lp_grad, loss.detach(), policy, loss2.detach(), margins, pref))
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
