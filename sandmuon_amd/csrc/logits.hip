@@ -259,8 +259,8 @@ struct LongRow {
 // Rows of a block and this thread's one; -1 where there is none.
 template <int NT>
 __device__ __forceinline__ int64_t row_of(int64_t rows) {
-  if constexpr (NT > 64) return blockIdx.x;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int64_t r = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+  if constexpr (NT == 64) r = r * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   return r < rows ? r : -1;
 }
 
@@ -507,6 +507,13 @@ static int logits_check(const char *what, const void *z, int dtype, int64_t batc
   return SMX_OK;
 }
 
+// A launch holds fewer than 2^32 threads along one axis, so the blocks of many
+// rows lie along two.
+static dim3 row_grid(int64_t blocks) {
+  const int64_t x = std::min<int64_t>(blocks, int64_t{1} << 20);
+  return dim3(static_cast<unsigned>(x), static_cast<unsigned>(ceil_div(blocks, x)));
+}
+
 // Threads and chunks by the row's length in 16-byte chunks: a wave a row (four
 // rows a block) up to 8 KB, so that a short row waits for no other wave; then
 // 256, 512 and 1024 threads with up to 16 chunks each, the fewest that hold
@@ -514,17 +521,17 @@ static int logits_check(const char *what, const void *z, int dtype, int64_t batc
 #define LOGITS_BY_ROW(DT, vocab, rows, NAME, ...)                                                                   \
   do {                                                                                                              \
     const int64_t chunks_ = ceil_div(vocab, Logit<DT>::kPer);                                                       \
-    const unsigned rows_ = static_cast<unsigned>(rows);                                                             \
+    const dim3 grid_ = row_grid(chunks_ <= 512 ? ceil_div(rows, 4) : (rows));                                       \
     if (chunks_ <= 512) {                                                                                           \
-      hipLaunchKernelGGL((NAME<DT, Row<DT, 64, 8>, 64>), dim3((rows_ + 3) / 4), dim3(256), 0, st, __VA_ARGS__);      \
+      hipLaunchKernelGGL((NAME<DT, Row<DT, 64, 8>, 64>), grid_, dim3(256), 0, st, __VA_ARGS__);                     \
     } else if (chunks_ <= 4096) {                                                                                   \
-      hipLaunchKernelGGL((NAME<DT, Row<DT, 256, 16>, 256>), dim3(rows_), dim3(256), 0, st, __VA_ARGS__);            \
+      hipLaunchKernelGGL((NAME<DT, Row<DT, 256, 16>, 256>), grid_, dim3(256), 0, st, __VA_ARGS__);                  \
     } else if (chunks_ <= 8192) {                                                                                   \
-      hipLaunchKernelGGL((NAME<DT, Row<DT, 512, 16>, 512>), dim3(rows_), dim3(512), 0, st, __VA_ARGS__);            \
+      hipLaunchKernelGGL((NAME<DT, Row<DT, 512, 16>, 512>), grid_, dim3(512), 0, st, __VA_ARGS__);                  \
     } else if (chunks_ <= 16384) {                                                                                  \
-      hipLaunchKernelGGL((NAME<DT, Row<DT, 1024, 16>, 1024>), dim3(rows_), dim3(1024), 0, st, __VA_ARGS__);         \
+      hipLaunchKernelGGL((NAME<DT, Row<DT, 1024, 16>, 1024>), grid_, dim3(1024), 0, st, __VA_ARGS__);               \
     } else {                                                                                                        \
-      hipLaunchKernelGGL((NAME<DT, LongRow<DT>, 1024>), dim3(rows_), dim3(1024), 0, st, __VA_ARGS__);               \
+      hipLaunchKernelGGL((NAME<DT, LongRow<DT>, 1024>), grid_, dim3(1024), 0, st, __VA_ARGS__);                     \
     }                                                                                                               \
   } while (0)
 

@@ -376,3 +376,14 @@ def test_rows_that_overlap(device, dtype):
             results.append((lp.detach(), lp_grad, loss.detach(), policy, loss2.detach(), margins, pref))
         for a, b in zip(*results):
             assert torch.equal(a, b)
+
+
+def test_more_rows_than_threads_along_one_axis(device):
+    # 2^26 waves of 64 are 2^32 threads
+    rows = (1 << 26) + 5
+    logits = torch.zeros(1, rows, 2, dtype=torch.float16, device=device)
+    logits[0, -1, 0] = 3
+    targets = torch.zeros(1, rows, dtype=torch.int64, device=device)
+    lp = losses.token_logprobs(logits, targets)[0]
+    assert lp[-1].item() == pytest.approx(-math.log1p(math.exp(-3)), rel=1e-6)
+    assert torch.equal(lp[:-1].min(), lp[:-1].max()) and lp[0].item() == pytest.approx(-math.log(2), rel=1e-6)
