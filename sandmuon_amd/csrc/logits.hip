@@ -506,7 +506,9 @@ __global__ void __launch_bounds__(1024) preference_kernel(PreferenceArgs a, int 
       for (int w = 1; w < share; ++w) gain += part[lead + w];
       // (the margin is rounded once; FP32 functions of it are within 2^-22)
       const float m = static_cast<float>(a.beta * gain), e = expf(-fabsf(m)), soft = log1pf(e);
-      loss += (1 - a.smoothing) * (soft - (m > 0.f ? 0.f : m)) + a.smoothing * (soft + (m < 0.f ? 0.f : m));
+      // (a term of weight zero is left out: it may be infinite)
+      if (a.smoothing < 1) loss += (1 - a.smoothing) * (soft - (m > 0.f ? 0.f : m));
+      if (a.smoothing > 0) loss += a.smoothing * (soft + (m < 0.f ? 0.f : m));
       a.margins[p] = m;
       // sigmoid(m) = 1 / (1 + e) or e / (1 + e)
       const double up = static_cast<double>(m > 0.f ? 1.f : e) / (1.0 + e);
@@ -647,6 +649,8 @@ extern "C" int smx_policy_loss(const void *logits, int dtype, int64_t batch, int
     a.logprobs = logprobs, a.weights = static_cast<float *>(workspace), a.terms = a.weights + batch, a.dz = dlogits;
     hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a, threads_of(batch, 16));
     LOGITS_LAUNCH(dtype, vocab, rows, policy_kernel, a);
+    const int lrc = check_launch("policy_loss");
+    if (lrc != SMX_OK) return lrc;
   }
   hipLaunchKernelGGL(sum_kernel, dim3(1), dim3(1024), 0, st, static_cast<const float *>(a.terms), rows, loss);
   return check_launch("policy_loss");

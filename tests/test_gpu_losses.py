@@ -387,3 +387,17 @@ def test_more_rows_than_threads_along_one_axis(device):
     lp = losses.token_logprobs(logits, targets)[0]
     assert lp[-1].item() == pytest.approx(-math.log1p(math.exp(-3)), rel=1e-6)
     assert torch.equal(lp[:-1].min(), lp[:-1].max()) and lp[0].item() == pytest.approx(-math.log(2), rel=1e-6)
+
+
+@pytest.mark.parametrize("v", [97, 5003])
+def test_preference_of_impossible_tokens(device, v):
+    # a target ruled out: an infinite margin for (loss 0) or against (loss inf) the chosen one
+    logits, targets, mask, _, ref, _ = make(device, 2, 5, v, torch.float32, 32)
+    for row, want in ((1, 0.0), (0, math.inf)):
+        leaf = logits.clone()
+        leaf[row, 2, targets[row, 2]] = -math.inf
+        leaf.requires_grad_()
+        loss, margins = losses.preference_loss(leaf, targets, ref, beta=0.3)
+        grad, = torch.autograd.grad(loss, leaf)
+        assert loss.item() == want and margins.item() == (math.inf if row else -math.inf)
+        assert torch.isfinite(grad).all() and grad.any().item() == (row == 0)
