@@ -216,11 +216,15 @@ std::tuple<Tensor, Tensor> qk_norm_rotary(Tensor q, Tensor k, OptTensor qw, OptT
     return {y[0], y[1]};
   }
   if (out.has_value()) {
-    for (const auto &[o, x] : {std::tie(std::get<0>(*out), q), std::tie(std::get<1>(*out), k)})
+    for (const auto &[o, x] : {std::tie(std::get<0>(*out), q), std::tie(std::get<1>(*out), k)}) {
       TORCH_CHECK_VALUE(o.sizes() == x.sizes() && o.scalar_type() == x.scalar_type() && o.device() == x.device() &&
                             (o.size(3) <= 1 || o.stride(3) == 1),
                         what, ": out ", o.sizes(), " ", o.scalar_type(), " for ", x.sizes(), " ", x.scalar_type(),
                         "; the last stride must be one");
+      for (int d = 0; d < 3; ++d)
+        TORCH_CHECK_VALUE(o.size(d) <= 1 || o.stride(d) != 0 || o.numel() == 0, what, ": out of strides ", o.strides(),
+                          " names places twice");
+    }
   } else {
     out = {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options())};
   }

@@ -238,3 +238,12 @@ def test_refusals(device):
         qk_norm_rotary(q.clone().requires_grad_(), k, qw, kw, cos, sin, out=(q, k))
     with pytest.raises(ValueError, match="eps"):
         qk_norm_rotary(q, k, qw, kw, cos, sin, eps=-1.0)
+
+
+def test_out_that_names_places_twice_is_refused(device):
+    q, k, qw, kw, cos, sin = make(device, 2, 3, 4, 1, 64, 64, torch.bfloat16, 13)
+    same = torch.empty(2, 3, 1, 64, dtype=q.dtype, device=device).expand(2, 3, 4, 64)
+    with pytest.raises(ValueError, match="twice"):
+        qk_norm_rotary(q, k, qw, kw, cos, sin, out=(same, torch.empty_like(k)))
+    y, z = qk_norm_rotary(q, k, qw, kw, cos, sin, out=(torch.empty_like(q), torch.empty_like(k)))
+    assert y.shape == q.shape and z.shape == k.shape
