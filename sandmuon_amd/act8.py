@@ -175,6 +175,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         _fmt(fmt, "act8.linear")
     elif _kept(kept, "act8.linear").shape != x.shape:
         raise ValueError(f"act8.linear: kept {tuple(kept.shape)} of an input {tuple(x.shape)}")
+    if not torch.is_grad_enabled():
+        return F.linear(x, weight, bias)
     return _Linear.apply(x, weight, bias, fmt, kept)
 
 
@@ -198,11 +200,14 @@ def gelu(h: torch.Tensor, fmt: str = "int8") -> torch.Tensor:
 
 class _Mlp(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, fc_w, fc_b, proj_w, proj_b, fmt):
+    def forward(ctx, x, fc_w, fc_b, proj_w, proj_b, fmt, grad):
+        # (only what the wanted gradients read is kept)
+        needs = [grad and need for need in ctx.needs_input_grad]
         x_lp, w1, b1, w2, b2 = (_cast(t, x.device.type) for t in (x, fc_w, fc_b, proj_w, proj_b))
         with torch.autocast(device_type=x.device.type, enabled=False):
-            ctx.kept_x = encode(x_lp, fmt)
-            y, ctx.kept_h, ctx.kept_y = gelu_forward(F.linear(x_lp, w1, b1), fmt)
+            ctx.kept_x = encode(x_lp, fmt) if needs[1] or needs[2] else None
+            y, kept_h, ctx.kept_y = gelu_forward(F.linear(x_lp, w1, b1), fmt, keep_output=needs[3] or needs[4])
+            ctx.kept_h = kept_h if any(needs[:3]) else None
             out = F.linear(y, w2, b2)
         ctx.save_for_backward(w1, w2)
         ctx.dtypes = tuple(None if t is None else t.dtype for t in (x, fc_w, fc_b, proj_w, proj_b))
@@ -213,10 +218,11 @@ class _Mlp(torch.autograd.Function):
     def backward(ctx, grad):
         w1, w2 = ctx.saved_tensors
         needs, types_ = ctx.needs_input_grad, ctx.dtypes
-        out = [None] * 6
+        out = [None] * 7
         if needs[3] or needs[4]:
             out[3], out[4] = linear_backward(grad, ctx.kept_y, types_[3], bias=needs[4])
-        dh = gelu_backward(_input_grad(grad, w2, grad.dtype), ctx.kept_h)
+        if any(needs[:3]):
+            dh = gelu_backward(_input_grad(grad, w2, grad.dtype), ctx.kept_h)
         if needs[1] or needs[2]:
             out[1], out[2] = linear_backward(dh, ctx.kept_x, types_[1], bias=needs[2])
         if needs[0]:
@@ -232,7 +238,7 @@ def mlp(x: torch.Tensor, fc_weight: torch.Tensor, fc_bias: Optional[torch.Tensor
     """proj(GELU(fc(x))) with x, the hidden layer and the GELU's output kept in
     8 bits: 1 byte an element where three 16-bit tensors would be kept."""
     _fmt(fmt, "act8.mlp")
-    return _Mlp.apply(x, fc_weight, fc_bias, proj_weight, proj_bias, fmt)
+    return _Mlp.apply(x, fc_weight, fc_bias, proj_weight, proj_bias, fmt, torch.is_grad_enabled())
 
 
 class CheckpointedLinears:

@@ -423,3 +423,30 @@ def test_gradients_of_sums_over_rows(device):
             grads.append((leaf.grad, weight.grad))
         for a, b in zip(*grads):
             assert (a is None and b is None) or torch.equal(a, b)
+
+
+def test_frozen_parts(device):
+    torch.manual_seed(2)
+    x = activation(70, 40, torch.float32, device, 25)
+    fc, proj = torch.nn.Linear(40, 64).to(device), torch.nn.Linear(64, 24).to(device)
+    params = [fc.weight, fc.bias, proj.weight, proj.bias]
+
+    def run(forward, wanted):
+        leaves = [t.detach().clone().requires_grad_(want) for t, want in zip([x] + params, wanted)]
+        y = forward(*leaves)
+        if any(wanted):
+            y.sum().backward()
+        return [y.detach()] + [t.grad for t in leaves]
+
+    mlp = lambda t, w1, b1, w2, b2: act8.mlp(t, w1, b1, w2, b2)
+    linear = lambda t, w1, b1, w2, b2: act8.linear(t, w1, b1)
+    for forward, used in ((mlp, 5), (linear, 3)):
+        whole = run(forward, [True] * 5)
+        for bits in range(2 ** used):
+            wanted = [bool(bits >> i & 1) for i in range(5)]
+            got = run(forward, wanted)
+            assert torch.equal(got[0], whole[0])
+            for want, a, b in zip(wanted, got[1:], whole[1:]):
+                assert torch.equal(a, b) if want else a is None
+        with torch.no_grad():
+            assert torch.equal(forward(x, *params), whole[0])
