@@ -347,10 +347,12 @@ struct PolicyArgs {
   void *dz;
 };
 
-// Threads of a block of 1024 that share one of `items` sequences, at least `least`.
-static int threads_of(int64_t items, int least) {
+// Threads of a block of 1024 that share one of `items` sequences of `seq`
+// tokens, `per` of them in flight in each: as many as leave none idle, at least
+// `least`.
+static int threads_of(int64_t items, int64_t seq, int per, int least) {
   int share = 1024;
-  while (share > least && 1024 / share < items) share /= 2;
+  while (share > least && (1024 / share < items || share / 2 * per >= seq)) share /= 2;
   return share;
 }
 
@@ -647,7 +649,7 @@ extern "C" int smx_policy_loss(const void *logits, int dtype, int64_t batch, int
     a.kl = static_cast<float>(kl_coef), a.scale = static_cast<float>(scale);
     a.per_sequence = reduction == SMX_MEAN_SEQUENCE;
     a.logprobs = logprobs, a.weights = static_cast<float *>(workspace), a.terms = a.weights + batch, a.dz = dlogits;
-    hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a, threads_of(batch, 16));
+    hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a, threads_of(batch, seq, 8, 16));
     LOGITS_LAUNCH(dtype, vocab, rows, policy_kernel, a);
     const int lrc = check_launch("policy_loss");
     if (lrc != SMX_OK) return lrc;
@@ -665,7 +667,7 @@ extern "C" int smx_preference_loss(const float *logprobs, const float *ref_logpr
   SMX_REQUIRE(pairs == 0 || seq == 0 || (logprobs && ref_logprobs), SMX_EINVAL, "preference_loss: null log probabilities");
   const PreferenceArgs a{logprobs, ref_logprobs, mask, pairs, seq, beta, label_smoothing, loss, margins, coef};
   hipLaunchKernelGGL(preference_kernel, dim3(1), dim3(1024), 0, static_cast<hipStream_t>(stream), a,
-                     threads_of(pairs, 64) / 64);
+                     threads_of(pairs, seq, 4, 64) / 64);
   return check_launch("preference_loss");
 }
 
