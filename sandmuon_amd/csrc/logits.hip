@@ -523,13 +523,24 @@ __global__ void __launch_bounds__(1024) preference_kernel(PreferenceArgs a, int 
   if (threadIdx.x == 0) *a.loss = static_cast<float>(a.pairs ? loss / a.pairs : 0.);
 }
 
-// x *= *scale, unless it is one.
+// x *= *scale, unless it is one, in 16-byte chunks and single elements behind
+// them.  8 x 1024 x 50257 bf16: 339 us, the copy's rate (element by
+// element 589 us).
 template <int DT>
-__global__ void __launch_bounds__(256) scale_kernel(void *x, int64_t n, const float *scale) {
+__global__ void __launch_bounds__(256) scale_kernel(void *x, int64_t n, int64_t chunks, const float *scale) {
+  using L = Logit<DT>;
   const float s = *scale;
   if (s == 1.f) return;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
-    store_any(x, DT, i, round_to(DT, load_elem<DT>(x, i) * s));
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
+  uint4 *p = static_cast<uint4 *>(x);
+  for (int64_t i = first; i < chunks; i += step) {
+    const uint4 c = p[i];
+    float v[L::kPer];
+#pragma unroll
+    for (int k = 0; k < L::kPer; ++k) v[k] = L::at(c, k) * s;
+    p[i] = L::pack(v);
+  }
+  for (int64_t i = chunks * L::kPer + first; i < n; i += step) store_any(x, DT, i, round_to(DT, load_elem<DT>(x, i) * s));
 }
 
 // ----------------------------------------------------------------- host ---
@@ -676,14 +687,15 @@ extern "C" int smx_scale(void *x, int dtype, int64_t n, const float *scale, void
   SMX_REQUIRE(n >= 0, SMX_ESHAPE, "scale: negative size");
   if (n == 0) return SMX_OK;
   SMX_REQUIRE(x && scale, SMX_EINVAL, "scale: null pointer");
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(4096, ceil_div(n, 256))));
+  const int64_t per = dtype == SMX_F32 ? 4 : 8, chunks = reinterpret_cast<uintptr_t>(x) % 16 == 0 ? n / per : 0;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(2048, ceil_div(chunks ? chunks : n, 256))));
   const auto st = static_cast<hipStream_t>(stream);
   if (dtype == SMX_F32) {
-    hipLaunchKernelGGL((scale_kernel<SMX_F32>), grid, dim3(256), 0, st, x, n, scale);
+    hipLaunchKernelGGL((scale_kernel<SMX_F32>), grid, dim3(256), 0, st, x, n, chunks, scale);
   } else if (dtype == SMX_BF16) {
-    hipLaunchKernelGGL((scale_kernel<SMX_BF16>), grid, dim3(256), 0, st, x, n, scale);
+    hipLaunchKernelGGL((scale_kernel<SMX_BF16>), grid, dim3(256), 0, st, x, n, chunks, scale);
   } else {
-    hipLaunchKernelGGL((scale_kernel<SMX_F16>), grid, dim3(256), 0, st, x, n, scale);
+    hipLaunchKernelGGL((scale_kernel<SMX_F16>), grid, dim3(256), 0, st, x, n, chunks, scale);
   }
   return check_launch("scale");
 }

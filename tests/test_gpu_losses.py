@@ -14,7 +14,7 @@ import math
 import pytest
 import torch
 
-from sandmuon_amd import losses
+from sandmuon_amd import _native, losses
 
 pytestmark = pytest.mark.gpu
 
@@ -401,3 +401,25 @@ def test_preference_of_impossible_tokens(device, v):
         grad, = torch.autograd.grad(loss, leaf)
         assert loss.item() == want and margins.item() == (math.inf if row else -math.inf)
         assert torch.isfinite(grad).all() and grad.any().item() == (row == 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n", [1, 7, 8, 1031, 1 << 20])
+def test_scale(device, dtype, n):
+    x = (torch.randn(n + 3, generator=torch.Generator().manual_seed(n)) * 10).to(dtype).to(device)
+    for at in (0, 3):  # (at 16-byte boundaries and off them)
+        for factor in (1.0, 0.37, -2.0 ** 20, 0.0, math.inf):
+            got = x.clone()
+            scale = torch.tensor([factor], device=device)
+            rc = _native.lib().smx_scale(got.data_ptr() + at * x.element_size(), _native.dtype_code(dtype), n,
+                                         scale.data_ptr(), _native.stream_of(x.device))
+            assert rc == 0
+            want = x.clone()
+            want[at:at + n] = (x[at:at + n].float() * factor).to(dtype)
+            if factor != 0.37:  # (exact products, rounded once)
+                assert torch.equal(torch.nan_to_num(got, nan=5.0), torch.nan_to_num(want, nan=5.0))
+                continue
+            # half a place of the type, and an FP32 rounding of the product where the kernel makes one
+            assert torch.equal(got[:at], x[:at]) and torch.equal(got[at + n:], x[at + n:])
+            exact = x[at:at + n].double() * scale.double()
+            assert ((got[at:at + n].double() - exact).abs() <= (PLACE[dtype] + 2.0 ** -24) * exact.abs() + 2.0 ** -25).all()
