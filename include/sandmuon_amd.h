@@ -656,7 +656,8 @@ int smx_policy_loss(const void *logits, int dtype, int64_t batch, int64_t seq,
  * chosen sequences first: with m = beta * (gain of the chosen - gain of the
  * rejected), gain the sum of a sequence's live logprobs - ref_logprobs,
  *   loss = mean of -(1 - s) log sigmoid(m) - s log sigmoid(-m),
- * s = label_smoothing; margins receives m, coef [2 * pairs] the derivative of
+ * s = label_smoothing (a part of weight zero is left out, infinite or not);
+ * margins receives m, coef [2 * pairs] the derivative of
  * the loss by a live token's log probability (smx_token_logprobs_backward's
  * coef with strides 1 and 0). */
 int smx_preference_loss(const float *logprobs, const float *ref_logprobs,

@@ -608,6 +608,7 @@ extern "C" int smx_token_logprobs(const void *logits, int dtype, int64_t batch, 
   const int rc = logits_check("token_logprobs", logits, dtype, batch, seq, vocab, batch_stride, row_stride, targets);
   if (rc != SMX_OK || batch * seq == 0) return rc;
   SMX_REQUIRE(logprobs, SMX_EINVAL, "token_logprobs: null output");
+  SMX_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, SMX_EALIGN, "token_logprobs: stats must be 8-byte aligned");
   const LogitRows a{logits, targets, mask, batch, seq, vocab, batch_stride, row_stride};
   const auto st = static_cast<hipStream_t>(stream);
   LOGITS_LAUNCH(dtype, vocab, batch * seq, logprob_kernel, a, logprobs, reinterpret_cast<float2 *>(stats));
@@ -622,6 +623,8 @@ extern "C" int smx_token_logprobs_backward(const void *logits, int dtype, int64_
   const int rc = logits_check("token_logprobs_backward", logits, dtype, batch, seq, vocab, batch_stride, row_stride, targets);
   if (rc != SMX_OK || batch * seq == 0) return rc;
   SMX_REQUIRE(stats && coef && dlogits, SMX_EINVAL, "token_logprobs_backward: null pointer");
+  SMX_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, SMX_EALIGN,
+              "token_logprobs_backward: stats must be 8-byte aligned");
   const LogitRows a{logits, targets, mask, batch, seq, vocab, batch_stride, row_stride};
   const CoefArgs k{reinterpret_cast<const float2 *>(stats), coef, scale, coef_batch_stride, coef_row_stride, dlogits};
   const auto st = static_cast<hipStream_t>(stream);

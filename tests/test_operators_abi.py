@@ -110,3 +110,9 @@ def test_loss_refusals():
     assert lib.smx_preference_loss(P, P, None, -1, 3, .1, 0.0, P, P, P, None) == -2
     assert lib.smx_scale(P, 4, 1, P, None) == -3 and lib.smx_scale(None, 1, 1, P, None) == -1
     assert lib.smx_scale(None, 1, 0, None, None) == 0
+
+
+def test_loss_stats_alignment():
+    lib = _native.lib()
+    assert lib.smx_token_logprobs(P, 1, 2, 3, 50, 150, 50, P, None, P, 260, None) == -4
+    assert lib.smx_token_logprobs_backward(P, 1, 2, 3, 50, 150, 50, P, None, 260, P, 3, 1, None, P, None) == -4
