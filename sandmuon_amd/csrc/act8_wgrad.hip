@@ -11,8 +11,9 @@
 // as the two or three BF16 parts that sum to them exactly, with a product each.
 //
 // The two LDS buffers alternate: beside one step's MFMAs the next step is
-// written to the other, and loads of a later step are in flight.  Splits of m write FP32 partial tiles that a second launch adds in
-// order, so the result does not depend on timing.
+// written to the other, and loads of a later step are in flight.  Splits of m
+// write FP32 partial tiles that a second launch adds in order, so the result
+// does not depend on timing.
 //
 // Measured, BF16 cotangents, with db: 8192 x 2048 -> 8192 253 us in e4m3 (1.09
 // PFLOP/s) and 287 us in int8, whose codes take 2.5 vector instructions an element

@@ -230,7 +230,9 @@ __global__ void __launch_bounds__(kQkThreads) qk_kernel(QkArgs a) {
       for (int e = threadIdx.x; e < 8 * G; e += kQkThreads) {
         const QkLane o = qk_lane<HALF>(a, e >> 3);
         const int k = e & 7;
-        if (o.active) part[(k < 4 ? o.lo : o.hi - 4) + k] = (red[0][e >> 3][k] + red[1][e >> 3][k]) + (red[2][e >> 3][k] + red[3][e >> 3][k]);
+        if (o.active)
+          part[(k < 4 ? o.lo : o.hi - 4) + k] =
+              (red[0][e >> 3][k] + red[1][e >> 3][k]) + (red[2][e >> 3][k] + red[3][e >> 3][k]);
       }
     }
   }
@@ -376,7 +378,9 @@ static QkPlan qk_plan(const smx_qk_desc &d, bool back) {
   for (int i = 0; i < 2; ++i) {
     const smx_qk_side &s = i ? d.k : d.q;
     const int64_t items = d.batch * d.seq * s.heads;
-    p.blocks[i] = items == 0 ? 0 : static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(items, per_block), ceil_div(want * items, all))));
+    p.blocks[i] = items == 0 ? 0
+                             : static_cast<int>(std::max<int64_t>(
+                                   1, std::min(ceil_div(items, per_block), ceil_div(want * items, all))));
     p.rows[i] = p.vec ? p.blocks[i] : 4 * p.blocks[i];
   }
   return p;
