@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define SMX_ABI_VERSION 6
+#define SMX_ABI_VERSION 7
 
 enum smx_status {
   SMX_OK = 0,
@@ -651,6 +651,23 @@ int smx_policy_loss(const void *logits, int dtype, int64_t batch, int64_t seq,
                     double kl_coef, int reduction, double scale, float *loss,
                     float *logprobs, void *dlogits, void *workspace,
                     int64_t workspace_bytes, void *stream);
+
+/* smx_policy_loss_coef: the same loss with no gradient; stats [batch, seq, 2]
+ * (8-byte aligned) and coef [batch, seq] receive what
+ * smx_token_logprobs_backward makes it from (coef strides seq and 1), times a
+ * factor given there, before the one rounding: for FP16 logits, whose
+ * gradient at unit scale mostly lies below FP16's smallest number. */
+int smx_policy_loss_coef(const void *logits, int dtype, int64_t batch,
+                         int64_t seq, int64_t vocab, int64_t batch_stride,
+                         int64_t row_stride, const int64_t *targets,
+                         const uint8_t *mask, const float *old_logprobs,
+                         const float *ref_logprobs, const float *advantages,
+                         int64_t adv_batch_stride, int64_t adv_row_stride,
+                         double clip_low, double clip_high, double kl_coef,
+                         int reduction, double scale, float *loss,
+                         float *logprobs, float *stats, float *coef,
+                         void *workspace, int64_t workspace_bytes,
+                         void *stream);
 
 /* smx_preference_loss: from token log probabilities [2 * pairs, seq], the
  * chosen sequences first: with m = beta * (gain of the chosen - gain of the

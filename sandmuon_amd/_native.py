@@ -18,7 +18,7 @@ from typing import List, Optional, Sequence
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libsandmuon_amd.so"
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 SMX_F32, SMX_BF16, SMX_F16, SMX_F64 = 0, 1, 2, 3
 S8_FP32, S8_COMP_BF16, S8_MIXED = 0, 1, 2
@@ -170,6 +170,9 @@ SIGNATURES.update({
     "smx_policy_loss_workspace_bytes": (c_int64, [c_int64, c_int64]),
     "smx_policy_loss": (c_int, [*_LOGITS, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_double, c_double, c_double,
                                 c_int, c_double, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "smx_policy_loss_coef": (c_int, [*_LOGITS, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_double, c_double,
+                                     c_double, c_int, c_double, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_int64, c_void_p]),
     "smx_preference_loss": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_double, c_double, c_void_p,
                                     c_void_p, c_void_p, c_void_p]),
     "smx_scale": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p]),

@@ -347,7 +347,9 @@ struct PolicyArgs {
   float low, high, kl, scale;  // the ratio's unclipped range
   int32_t per_sequence;
   float *logprobs, *weights, *terms;  // [batch, seq], [batch], [batch, seq]
-  void *dz;
+  void *dz;                           // the gradient, or null
+  float2 *stats;                      // or, for one made later, each row's maximum and sum
+  float *coef;                        // and d loss / d lp
 };
 
 // Threads of a block of 1024 that share one of `items` sequences of `seq`
@@ -418,12 +420,19 @@ ROW_KERNEL(R, NT, policy_kernel, PolicyArgs a) {
   const int64_t b = r / q.seq, t = r % q.seq;
   R row;
   if (q.mask && !q.mask[r]) {
-    if (lane == 0) a.logprobs[r] = a.terms[r] = 0.f;
+    if (lane == 0) {
+      a.logprobs[r] = a.terms[r] = 0.f;
+      if (a.coef) a.stats[r] = make_float2(0.f, 1.f), a.coef[r] = 0.f;
+    }
     if (a.dz) row.zero(a.dz, r * q.vocab, q.vocab);
     return;
   }
   const int64_t at = b * q.batch_stride + t * q.row_stride, y = q.targets[r];
-  row.template load<false>(q.z, at, q.vocab);
+  if (a.coef) {
+    row.template load<true>(q.z, at, q.vocab);
+  } else {
+    row.template load<false>(q.z, at, q.vocab);
+  }
   const RowStat o = row.stat(scratch);
   const float lp = target_lp<DT>(q, at, y, o);
   const float w = a.weights[b], adv = a.adv[b * a.adv_batch + t * a.adv_seq];
@@ -441,6 +450,7 @@ ROW_KERNEL(R, NT, policy_kernel, PolicyArgs a) {
   if (lane == 0) {
     a.logprobs[r] = lp;
     a.terms[r] = w * term;
+    if (a.coef) a.stats[r] = make_float2(o.top, o.sum), a.coef[r] = w * c;
   }
   if (a.dz) row.grad(a.dz, r * q.vocab, y < q.vocab ? y : -1, o, w * c);
 }
@@ -640,39 +650,77 @@ extern "C" int64_t smx_policy_loss_workspace_bytes(int64_t batch, int64_t seq) {
   return (batch + batch * seq) * static_cast<int64_t>(sizeof(float));
 }
 
+namespace smx {
+// What both entry points take: logits and targets, the policies' log probabilities, the loss.
+struct PolicyCall {
+  LogitRows rows;
+  int dtype;
+  const float *old_lp, *ref_lp, *adv;
+  int64_t adv_batch, adv_seq;
+  double clip_low, clip_high, kl, scale;
+  int reduction;
+  float *loss, *logprobs;
+  void *workspace;
+  int64_t workspace_bytes;
+};
+
+static int policy_run(const char *what, const PolicyCall &c, void *dz, float *stats, float *coef, hipStream_t st) {
+  const auto msg = [&](const char *m) { return std::string(what) + ": " + m; };
+  const LogitRows &q = c.rows;
+  const int rc = logits_check(what, q.z, c.dtype, q.batch, q.seq, q.vocab, q.batch_stride, q.row_stride, q.targets);
+  if (rc != SMX_OK) return rc;
+  SMX_REQUIRE(c.reduction == SMX_MEAN_TOKEN || c.reduction == SMX_MEAN_SEQUENCE, SMX_EINVAL, msg("unknown reduction"));
+  SMX_REQUIRE(c.clip_low >= 0 && c.clip_low <= 1 && c.clip_high >= 0, SMX_EINVAL,
+              msg("clip_low must be in [0, 1] and clip_high not negative"));
+  SMX_REQUIRE(c.loss, SMX_EINVAL, msg("null loss"));
+  const int64_t rows = q.batch * q.seq;
+  PolicyArgs a{};
+  if (rows > 0) {
+    SMX_REQUIRE(c.logprobs && c.adv, SMX_EINVAL, msg("null pointer"));
+    SMX_REQUIRE(c.workspace && c.workspace_bytes >= smx_policy_loss_workspace_bytes(q.batch, q.seq), SMX_EWORKSPACE,
+                msg("workspace too small"));
+    a.rows = q, a.old_lp = c.old_lp, a.ref_lp = c.ref_lp, a.adv = c.adv;
+    a.adv_batch = c.adv_batch, a.adv_seq = c.adv_seq;
+    a.low = static_cast<float>(1 - c.clip_low), a.high = static_cast<float>(1 + c.clip_high);
+    a.kl = static_cast<float>(c.kl), a.scale = static_cast<float>(c.scale);
+    a.per_sequence = c.reduction == SMX_MEAN_SEQUENCE;
+    a.logprobs = c.logprobs, a.weights = static_cast<float *>(c.workspace), a.terms = a.weights + q.batch;
+    a.dz = dz, a.stats = reinterpret_cast<float2 *>(stats), a.coef = coef;
+    hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a, threads_of(q.batch, q.seq, 8, 16));
+    LOGITS_LAUNCH(c.dtype, q.vocab, rows, policy_kernel, a);
+    const int lrc = check_launch(what);
+    if (lrc != SMX_OK) return lrc;
+  }
+  hipLaunchKernelGGL(sum_kernel, dim3(1), dim3(1024), 0, st, static_cast<const float *>(a.terms), rows, c.loss);
+  return check_launch(what);
+}
+}  // namespace smx
+
 extern "C" int smx_policy_loss(const void *logits, int dtype, int64_t batch, int64_t seq, int64_t vocab,
                                int64_t batch_stride, int64_t row_stride, const int64_t *targets, const uint8_t *mask,
                                const float *old_logprobs, const float *ref_logprobs, const float *advantages,
                                int64_t adv_batch_stride, int64_t adv_row_stride, double clip_low, double clip_high,
                                double kl_coef, int reduction, double scale, float *loss, float *logprobs,
                                void *dlogits, void *workspace, int64_t workspace_bytes, void *stream) {
-  const int rc = logits_check("policy_loss", logits, dtype, batch, seq, vocab, batch_stride, row_stride, targets);
-  if (rc != SMX_OK) return rc;
-  SMX_REQUIRE(reduction == SMX_MEAN_TOKEN || reduction == SMX_MEAN_SEQUENCE, SMX_EINVAL, "policy_loss: unknown reduction");
-  SMX_REQUIRE(clip_low >= 0 && clip_low <= 1 && clip_high >= 0, SMX_EINVAL,
-              "policy_loss: clip_low must be in [0, 1] and clip_high not negative");
-  SMX_REQUIRE(loss, SMX_EINVAL, "policy_loss: null loss");
-  const auto st = static_cast<hipStream_t>(stream);
-  const int64_t rows = batch * seq;
-  PolicyArgs a{};
-  if (rows > 0) {
-    SMX_REQUIRE(logprobs && advantages, SMX_EINVAL, "policy_loss: null pointer");
-    SMX_REQUIRE(workspace && workspace_bytes >= smx_policy_loss_workspace_bytes(batch, seq), SMX_EWORKSPACE,
-                "policy_loss: workspace too small");
-    a.rows = {logits, targets, mask, batch, seq, vocab, batch_stride, row_stride};
-    a.old_lp = old_logprobs, a.ref_lp = ref_logprobs, a.adv = advantages;
-    a.adv_batch = adv_batch_stride, a.adv_seq = adv_row_stride;
-    a.low = static_cast<float>(1 - clip_low), a.high = static_cast<float>(1 + clip_high);
-    a.kl = static_cast<float>(kl_coef), a.scale = static_cast<float>(scale);
-    a.per_sequence = reduction == SMX_MEAN_SEQUENCE;
-    a.logprobs = logprobs, a.weights = static_cast<float *>(workspace), a.terms = a.weights + batch, a.dz = dlogits;
-    hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a, threads_of(batch, seq, 8, 16));
-    LOGITS_LAUNCH(dtype, vocab, rows, policy_kernel, a);
-    const int lrc = check_launch("policy_loss");
-    if (lrc != SMX_OK) return lrc;
-  }
-  hipLaunchKernelGGL(sum_kernel, dim3(1), dim3(1024), 0, st, static_cast<const float *>(a.terms), rows, loss);
-  return check_launch("policy_loss");
+  const PolicyCall c{{logits, targets, mask, batch, seq, vocab, batch_stride, row_stride}, dtype, old_logprobs,
+                     ref_logprobs, advantages, adv_batch_stride, adv_row_stride, clip_low, clip_high, kl_coef, scale,
+                     reduction, loss, logprobs, workspace, workspace_bytes};
+  return policy_run("policy_loss", c, dlogits, nullptr, nullptr, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int smx_policy_loss_coef(const void *logits, int dtype, int64_t batch, int64_t seq, int64_t vocab,
+                                    int64_t batch_stride, int64_t row_stride, const int64_t *targets,
+                                    const uint8_t *mask, const float *old_logprobs, const float *ref_logprobs,
+                                    const float *advantages, int64_t adv_batch_stride, int64_t adv_row_stride,
+                                    double clip_low, double clip_high, double kl_coef, int reduction, double scale,
+                                    float *loss, float *logprobs, float *stats, float *coef, void *workspace,
+                                    int64_t workspace_bytes, void *stream) {
+  const PolicyCall c{{logits, targets, mask, batch, seq, vocab, batch_stride, row_stride}, dtype, old_logprobs,
+                     ref_logprobs, advantages, adv_batch_stride, adv_row_stride, clip_low, clip_high, kl_coef, scale,
+                     reduction, loss, logprobs, workspace, workspace_bytes};
+  SMX_REQUIRE((stats && coef) || batch == 0 || seq == 0, SMX_EINVAL, "policy_loss_coef: null stats or coef");
+  SMX_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, SMX_EALIGN, "policy_loss_coef: stats must be 8-byte aligned");
+  return policy_run("policy_loss_coef", c, nullptr, stats, coef, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int smx_preference_loss(const float *logprobs, const float *ref_logprobs, const uint8_t *mask,

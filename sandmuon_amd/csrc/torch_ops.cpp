@@ -324,37 +324,64 @@ Tensor token_logprobs(Tensor logits, Tensor targets, OptTensor mask) {
 }
 
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+  // The gradient of FP32 and BF16 logits is made with the loss, in the pass that
+  // reads them.  Of FP16 ones, at unit scale, most would round to zero before a
+  // loss scaler's factor arrives: theirs is made in the backward, and rounded once
+  // with the factor in it.
   static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &targets, const OptTensor &mask,
                                const OptTensor &old, const OptTensor &ref, const Tensor &adv, double low, double high,
                                double kl, int64_t reduction, double scale, bool want_grad) {
     const Tensor loss = fp32(logits, {}), lp = fp32(logits, targets.sizes());
-    Tensor grad;
-    if (want_grad) grad = at::empty(logits.sizes(), logits.options());
+    const bool later = want_grad && logits.scalar_type() == torch::kFloat16;
+    Tensor grad, stats, coef;
+    if (later) {
+      stats = fp32(logits, {targets.size(0), targets.size(1), 2}), coef = fp32(logits, targets.sizes());
+    } else if (want_grad) {
+      grad = at::empty(logits.sizes(), logits.options());
+    }
     const Rows r = rows_of(logits, targets, mask);
     const int64_t bytes = smx_policy_loss_workspace_bytes(r.batch, r.seq);
     const Tensor work = at::empty({bytes}, logits.options().dtype(torch::kUInt8));
     const c10::DeviceGuard guard(logits.device());
-    check(smx_policy_loss(ROWS(r), ptr<float>(old), ptr<float>(ref), adv.data_ptr<float>(), adv.stride(0),
-                          adv.dim() == 2 ? adv.stride(1) : 0, low, high, kl, static_cast<int>(reduction), scale,
-                          loss.data_ptr<float>(), lp.data_ptr<float>(), want_grad ? grad.data_ptr() : nullptr,
-                          work.data_ptr(), bytes, stream_of(logits)),
-          "smx_policy_loss");
+#define POLICY(r)                                                                                             \
+  ROWS(r), ptr<float>(old), ptr<float>(ref), adv.data_ptr<float>(), adv.stride(0),                            \
+      adv.dim() == 2 ? adv.stride(1) : 0, low, high, kl, static_cast<int>(reduction), scale, loss.data_ptr<float>(), \
+      lp.data_ptr<float>()
+    if (later) {
+      check(smx_policy_loss_coef(POLICY(r), stats.data_ptr<float>(), coef.data_ptr<float>(), work.data_ptr(), bytes,
+                                 stream_of(logits)),
+            "smx_policy_loss_coef");
+    } else {
+      check(smx_policy_loss(POLICY(r), want_grad ? grad.data_ptr() : nullptr, work.data_ptr(), bytes, stream_of(logits)),
+            "smx_policy_loss");
+    }
+#undef POLICY
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({lp});
-    if (want_grad) ctx->saved_data["grad"] = grad;
+    ctx->saved_data["later"] = later;
+    if (later) {
+      ctx->save_for_backward({logits, targets, mask.value_or(Tensor()), stats, coef});
+    } else if (want_grad) {
+      ctx->saved_data["grad"] = grad;
+    }
     return {loss, lp};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     no_double_backward("policy_loss");
     variable_list out(12);
     if (!grads[0].defined()) return out;
+    const Tensor scale = grads[0].to(torch::kFloat32);
+    if (ctx->saved_data["later"].toBool()) {
+      const auto s = ctx->get_saved_variables();
+      out[0] = logprobs_backward(s[0], s[1], some(s[2]), s[3], s[4], s[4].stride(0), s[4].stride(1), scale);
+      return out;
+    }
     const auto it = ctx->saved_data.find("grad");
     TORCH_CHECK(it != ctx->saved_data.end(),
                 "policy_loss: the gradient is made with the loss and handed out once; call policy_loss again to go "
                 "through it a second time");
     out[0] = it->second.toTensor();
     ctx->saved_data.erase(it);
-    const Tensor scale = grads[0].to(torch::kFloat32);
     const c10::DeviceGuard guard(out[0].device());
     check(smx_scale(out[0].data_ptr(), dtype_of(out[0]), out[0].numel(), scale.data_ptr<float>(), stream_of(out[0])),
           "smx_scale");

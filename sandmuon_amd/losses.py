@@ -43,10 +43,12 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
     means ("sequence"), times `scale`; 0 where no token is live.  advantages:
     [batch] or [batch, seq].  logprobs is lp, not differentiable.
 
-    The gradient to the logits is made in the pass that reads them.  Backward
-    of another factor than 1 costs a pass over it and a second rounding: give a
-    constant factor (one over the accumulated batches) as `scale`.  It can be
-    gone through once."""
+    The gradient to float32 and bfloat16 logits is made in the pass that reads
+    them.  Backward of another factor than 1 costs a pass over it and a second
+    rounding: give a constant factor (one over the accumulated batches) as
+    `scale`.  It can be gone through once.  The gradient to float16 logits is
+    made in the backward, from a second read of them, and a loss scaler's
+    factor enters it before its one rounding."""
     code = REDUCTIONS.get(reduction)
     if code is None:
         raise ValueError(f"policy_loss: unknown reduction {reduction!r}; expected one of {sorted(REDUCTIONS)}")

@@ -116,3 +116,16 @@ def test_loss_stats_alignment():
     lib = _native.lib()
     assert lib.smx_token_logprobs(P, 1, 2, 3, 50, 150, 50, P, None, P, 260, None) == -4
     assert lib.smx_token_logprobs_backward(P, 1, 2, 3, 50, 150, 50, P, None, 260, P, 3, 1, None, P, None) == -4
+
+
+def test_policy_loss_coef_refusals():
+    lib = _native.lib()
+
+    def call(z=P, low=.2, reduction=0, loss=P, adv=P, stats=P, coef=P, work=P, bytes_=1 << 20, batch=2):
+        return lib.smx_policy_loss_coef(z, 2, batch, 3, 50, 150, 50, P, None, None, None, adv, 1, 0, low, .2, 0.0, reduction,
+                                        1.0, loss, P, stats, coef, work, bytes_, None)
+
+    assert call(z=None) == -1 and call(low=-.1) == -1 and call(reduction=2) == -1 and call(loss=None) == -1
+    assert call(adv=None) == -1 and call(stats=None) == -1 and call(coef=None) == -1 and call(stats=ctypes.c_void_p(260)) == -4
+    assert call(work=None) == -5 and call(bytes_=4) == -5 and call(batch=-1) == -2
+    assert b"policy_loss_coef" in lib.smx_last_error()
