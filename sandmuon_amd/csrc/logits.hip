@@ -436,7 +436,8 @@ ROW_KERNEL(R, NT, policy_kernel, PolicyArgs a) {
   const RowStat o = row.stat(scratch);
   const float lp = target_lp<DT>(q, at, y, o);
   const float w = a.weights[b], adv = a.adv[b * a.adv_batch + t * a.adv_seq];
-  const float ratio = a.old_lp ? expf(lp - a.old_lp[r]) : 1.f;
+  const bool known = y >= 0 && y < q.vocab;
+  const float ratio = a.old_lp ? expf(lp - a.old_lp[r]) : known ? 1.f : __builtin_nanf("");
   // (comparisons that keep a NaN, which fminf and fmaxf would drop)
   const float clipped = ratio < a.low ? a.low : ratio > a.high ? a.high : ratio;
   float term = -(clipped * adv < ratio * adv ? clipped * adv : ratio * adv);
@@ -447,6 +448,8 @@ ROW_KERNEL(R, NT, policy_kernel, PolicyArgs a) {
     term += a.kl * (em1 - gap);
     c -= a.kl * em1;
   }
+  // (a comparison drops a NaN that the term has, or its part of c is zero)
+  if (!known || term != term) c = __builtin_nanf("");
   if (lane == 0) {
     a.logprobs[r] = lp;
     a.terms[r] = w * term;
