@@ -547,7 +547,8 @@ int smx_act8_gelu_backward(const void *dy, int dtype, int64_t rows,
  * db[n] = sum over rows of delta[row, n] (db may be null), both contiguous of
  * `out_dtype`, rounded once from FP32 sums.  Products are exact: a BF16
  * delta times a code's value; an FP16 or FP32 delta as the sum of its two or
- * three BF16 parts.  rows = 0 gives zeros.  `workspace`: 256-byte aligned,
+ * three BF16 parts (an FP32 one's bits below 2^-133, BF16's smallest number,
+ * are dropped).  rows = 0 gives zeros.  `workspace`: 256-byte aligned,
  * smx_act8_wgrad_workspace_bytes(rows, n, k, dtype) bytes (none needed: 0). */
 int64_t smx_act8_wgrad_workspace_bytes(int64_t rows, int64_t n, int64_t k,
                                        int dtype);

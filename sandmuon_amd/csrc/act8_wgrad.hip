@@ -1,14 +1,15 @@
 // The weight and bias gradients of a Linear whose input is kept in 8 bits:
 //   dW[n, k] = sum_m delta[m, n] * held(x)[m, k],   db[n] = sum_m delta[m, n].
 //
-// One block of four waves owns a T x T tile of dW over a range of rows m (a
-// split) and goes over it in steps of kStep rows.  Both operands have the sum's
-// index m as their slow axis, so each step is staged row by row in LDS as BF16
-// and read back transposed (ds_read_b64_tr_b16: four rows of one column per
-// lane) as the operands of v_mfma_f32_32x32x16_bf16.  The codes become BF16 on
-// the way into LDS: a code times its scale is exact in BF16, so its product
-// with a BF16 cotangent is exact in FP32.  FP16 and FP32 cotangents are staged
-// as the two or three BF16 parts that sum to them exactly, with a product each.
+// One block owns a tile of dW (256 x 256 by eight waves, or 128 x 128 by four)
+// over a range of rows m (a split) and goes over it in steps of kStep rows.  Both
+// operands have the sum's index m as their slow axis, so each step is staged row
+// by row in LDS as BF16 and read back transposed (ds_read_b64_tr_b16: four rows of
+// one column per lane) as the operands of v_mfma_f32_32x32x16_bf16.  The codes
+// become BF16 on the way into LDS: a code times its scale is exact in BF16, so its
+// product with a BF16 cotangent is exact in FP32.  FP16 and FP32 cotangents are
+// staged as the two or three BF16 parts that sum to them (down to 2^-133), with a
+// product each.
 //
 // The two LDS buffers alternate: beside one step's MFMAs the next step is
 // written to the other, and loads of a later step are in flight.  Splits of m
@@ -64,12 +65,10 @@ __device__ __forceinline__ void act8_to_bf16(const uint4 &c, int b, uint4 *o) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     if constexpr (FMT == SMX_ACT8_INT8) {
-      // (code + 128) scale - 128 scale, exact; the upper halves are the BF16 values
-      const uint32_t u = w[q] ^ 0x80808080u;
+      // code * scale, exact; the upper halves are the BF16 values
       float f[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        f[k] = fmaf(static_cast<float>((u >> (8 * k)) & 255u), scale, -128.f * scale);
+      for (int k = 0; k < 4; ++k) f[k] = static_cast<float>(static_cast<int8_t>(w[q] >> (8 * k))) * scale;
       r[2 * q] = __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u);
       r[2 * q + 1] = __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u);
     } else {
@@ -110,8 +109,8 @@ struct Cot8 {
     if constexpr (DT == SMX_BF16) return __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
     return f16_bits_to_f32(static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1))));
   }
-  // Its BF16 parts: each the leading eight bits of what is left (exact), the
-  // rest of an infinity being nothing.
+  // Its BF16 parts: each the leading eight bits of what is left (exact down to
+  // 2^-133, BF16's smallest number), the rest of an infinity being nothing.
   __device__ __forceinline__ void parts(uint4 *o) const {
     if constexpr (DT == SMX_BF16) {
       o[0] = make_uint4(w[0], w[1], w[2], w[3]);

@@ -1,5 +1,5 @@
 """The weight gradient on sizes that take its 256 x 256 tiles (those of the other
-tests stay on 128 x 128 ones), and infinities and NaN in both formats.
+tests stay on 128 x 128 ones), and at the ends of the kept values' range.
 
 Bars as for the small sizes: products are exact and sums FP32, so each element is
 within (rows + 8) 2^-24 of the sum of its terms' magnitudes, plus one place of the
@@ -67,3 +67,19 @@ def test_infinities_and_nans(device, rows, k, n, dtype, fmt):
     assert torch.isnan(dw[12]).all() and not torch.isfinite(dw[9]).any()
     assert torch.isfinite(dw[rest][:, 64:]).all()
     assert db[9] == math.inf and torch.isnan(db[12]) and torch.isfinite(db[rest]).all()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,k,n", [(40, 96, 24), (515, 4001, 4090)])
+def test_blocks_at_the_ends_of_the_range(device, rows, k, n, dtype, fmt):
+    # the largest exponent (3e38) and the least (1e-38) in blocks of their own, beside ordinary ones
+    x = make(device, rows, k, torch.float32, 6)
+    x[3, :32] = torch.linspace(-1, 1, 32, device=device) * 3.3e38
+    x[4, 32:64] = torch.linspace(-1, 1, 32, device=device) * 1.6e38
+    x[5, :32] = torch.linspace(-1, 1, 32, device=device) * 1e-38
+    delta = make(device, rows, n, dtype, 7)
+    delta[3] *= 1e-36
+    delta[4] *= 1e-36
+    delta[3, ::2] = 0
+    check(delta, act8.encode(x.to(dtype), fmt), torch.float32)
