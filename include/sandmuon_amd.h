@@ -549,7 +549,8 @@ int smx_act8_gelu_backward(const void *dy, int dtype, int64_t rows,
  * delta times a code's value; an FP16 or FP32 delta as the sum of its two or
  * three BF16 parts (an FP32 one's bits below 2^-133, BF16's smallest number,
  * are dropped).  rows = 0 gives zeros.  `workspace`: 256-byte aligned,
- * smx_act8_wgrad_workspace_bytes(rows, n, k, dtype) bytes (none needed: 0). */
+ * smx_act8_wgrad_workspace_bytes(rows, n, k, dtype) bytes (none needed: 0; n
+ * or k above 2^20: SMX_ESHAPE, as smx_act8_wgrad). */
 int64_t smx_act8_wgrad_workspace_bytes(int64_t rows, int64_t n, int64_t k,
                                        int dtype);
 int smx_act8_wgrad(const void *delta, int dtype, int64_t rows, int64_t n,

@@ -133,7 +133,7 @@ def _cast(t: Optional[torch.Tensor], device_type: str) -> Optional[torch.Tensor]
 
 
 def _input_grad(grad: torch.Tensor, weight: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    g2 = grad.reshape(-1, grad.shape[-1])
+    g2 = grad.reshape(grad.shape[:-1].numel(), grad.shape[-1])
     return g2.mm(weight).view(*grad.shape[:-1], weight.shape[1]).to(dtype)
 
 

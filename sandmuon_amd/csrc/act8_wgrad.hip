@@ -503,6 +503,8 @@ using namespace smx;
 
 extern "C" int64_t smx_act8_wgrad_workspace_bytes(int64_t rows, int64_t n, int64_t k, int dtype) {
   if (rows < 0 || n < 0 || k < 0 || dtype < SMX_F32 || dtype > SMX_F16) return SMX_EINVAL;
+  if (n > (int64_t{1} << 20) || k > (int64_t{1} << 20)) return SMX_ESHAPE;
+  if (n == 0) return 0;  // (no tile, nothing to plan)
   const WgradPlan p = wgrad_plan(dtype, rows, n, k);
   // the splits' partial tiles where there are several, and the parts of db
   const int64_t tiles = p.splits > 1 ? p.splits * n * k : 0, db = static_cast<int64_t>(p.splits) * p.tiles_k * n;

@@ -13,6 +13,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -557,7 +558,8 @@ std::tuple<Tensor, OptTensor> act8_linear_backward(const Tensor &delta, const Te
   const Tensor dw = at::empty({n, k.cols}, out);
   OptTensor db;
   if (bias) db = at::empty({n}, out);
-  const int64_t bytes = smx_act8_wgrad_workspace_bytes(k.rows, n, k.cols, dtype_of(r));
+  // (a refusal is the call's below)
+  const int64_t bytes = std::max<int64_t>(0, smx_act8_wgrad_workspace_bytes(k.rows, n, k.cols, dtype_of(r)));
   const Tensor work = at::empty({bytes}, r.options().dtype(torch::kUInt8));
   const c10::DeviceGuard guard(r.device());
   check(smx_act8_wgrad(r.data_ptr(), dtype_of(r), k.rows, n, r.stride(0), k.codes(), k.scales(), static_cast<int>(fmt),

@@ -129,3 +129,14 @@ def test_policy_loss_coef_refusals():
     assert call(adv=None) == -1 and call(stats=None) == -1 and call(coef=None) == -1 and call(stats=ctypes.c_void_p(260)) == -4
     assert call(work=None) == -5 and call(bytes_=4) == -5 and call(batch=-1) == -2
     assert b"policy_loss_coef" in lib.smx_last_error()
+
+
+def test_weight_gradient_of_no_outputs():
+    lib = _native.lib()
+    for k in (0, 40, 4096):
+        for dtype in (0, 1, 2):
+            assert lib.smx_act8_wgrad_workspace_bytes(4, 0, k, dtype) == 0
+    assert lib.smx_act8_wgrad_workspace_bytes(4, 8, 0, 1) >= 0 and lib.smx_act8_wgrad_workspace_bytes(0, 8, 40, 1) >= 0
+    # more features than a call takes: refused before the plan's products overflow
+    for n, k in ((1 << 21, 8), (8, 1 << 21), (1 << 40, 1 << 40)):
+        assert lib.smx_act8_wgrad_workspace_bytes(4, n, k, 1) == -2
