@@ -137,6 +137,13 @@ def _input_grad(grad: torch.Tensor, weight: torch.Tensor, dtype: torch.dtype) ->
     return g2.mm(weight).view(*grad.shape[:-1], weight.shape[1]).to(dtype)
 
 
+# The kept bytes are saved as tensors, so that a node's backward frees them (what
+# hangs on ctx lives as long as the graph, through the next step's forward where
+# the loss is still referred to) and saved-tensor hooks see them.
+def _data(saved: Optional[Act8]) -> Optional[torch.Tensor]:
+    return None if saved is None else saved.data
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, fmt, kept):
@@ -144,23 +151,25 @@ class _Linear(torch.autograd.Function):
         with torch.autocast(device_type=x.device.type, enabled=False):
             y = F.linear(x_lp, w, b)
         needs = ctx.needs_input_grad
-        if kept is None and (needs[1] or needs[2]):
+        if not (needs[1] or needs[2]):
+            kept = None
+        elif kept is None:
             kept = encode(x_lp, fmt)
-        ctx.kept = kept
-        ctx.save_for_backward(w)
+        ctx.save_for_backward(w if needs[0] else None, _data(kept))
+        ctx.kept = None if kept is None else (kept.shape, kept.fmt)
         ctx.dtypes = x.dtype, weight.dtype, None if bias is None else bias.dtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        w, = ctx.saved_tensors
+        w, data = ctx.saved_tensors
         x_dtype, w_dtype, b_dtype = ctx.dtypes
         needs = ctx.needs_input_grad
         dx = _input_grad(grad, w, x_dtype) if needs[0] else None
         dw = db = None
         if needs[1] or needs[2]:
-            dw, db = linear_backward(grad, ctx.kept, w_dtype, bias=needs[2])
+            dw, db = linear_backward(grad, Act8(data, *ctx.kept), w_dtype, bias=needs[2])
             if db is not None and b_dtype != w_dtype:
                 db = db.to(b_dtype)
         return dx, dw if needs[1] else None, db, None, None
@@ -183,13 +192,15 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 class _Gelu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, fmt):
-        y, ctx.kept, _ = gelu_forward(h, fmt, keep_output=False)
+        y, kept, _ = gelu_forward(h, fmt, keep_output=False)
+        ctx.save_for_backward(kept.data)
+        ctx.kept = kept.shape, kept.fmt
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        return gelu_backward(grad, ctx.kept), None
+        return gelu_backward(grad, Act8(*ctx.saved_tensors, *ctx.kept)), None
 
 
 def gelu(h: torch.Tensor, fmt: str = "int8") -> torch.Tensor:
@@ -205,26 +216,29 @@ class _Mlp(torch.autograd.Function):
         needs = [grad and need for need in ctx.needs_input_grad]
         x_lp, w1, b1, w2, b2 = (_cast(t, x.device.type) for t in (x, fc_w, fc_b, proj_w, proj_b))
         with torch.autocast(device_type=x.device.type, enabled=False):
-            ctx.kept_x = encode(x_lp, fmt) if needs[1] or needs[2] else None
-            y, kept_h, ctx.kept_y = gelu_forward(F.linear(x_lp, w1, b1), fmt, keep_output=needs[3] or needs[4])
-            ctx.kept_h = kept_h if any(needs[:3]) else None
+            kept_x = encode(x_lp, fmt) if needs[1] or needs[2] else None
+            y, kept_h, kept_y = gelu_forward(F.linear(x_lp, w1, b1), fmt, keep_output=needs[3] or needs[4])
+            if not any(needs[:3]):
+                kept_h = None
             out = F.linear(y, w2, b2)
-        ctx.save_for_backward(w1, w2)
+        ctx.save_for_backward(w1 if needs[0] else None, w2 if any(needs[:3]) else None, *map(_data, (kept_x, kept_h, kept_y)))
+        ctx.shapes, ctx.fmt = (x.shape, y.shape), fmt
         ctx.dtypes = tuple(None if t is None else t.dtype for t in (x, fc_w, fc_b, proj_w, proj_b))
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        w1, w2 = ctx.saved_tensors
+        w1, w2, x8, h8, y8 = ctx.saved_tensors
         needs, types_ = ctx.needs_input_grad, ctx.dtypes
+        of_x, of_h = ctx.shapes
         out = [None] * 7
         if needs[3] or needs[4]:
-            out[3], out[4] = linear_backward(grad, ctx.kept_y, types_[3], bias=needs[4])
+            out[3], out[4] = linear_backward(grad, Act8(y8, of_h, ctx.fmt), types_[3], bias=needs[4])
         if any(needs[:3]):
-            dh = gelu_backward(_input_grad(grad, w2, grad.dtype), ctx.kept_h)
+            dh = gelu_backward(_input_grad(grad, w2, grad.dtype), Act8(h8, of_h, ctx.fmt))
         if needs[1] or needs[2]:
-            out[1], out[2] = linear_backward(dh, ctx.kept_x, types_[1], bias=needs[2])
+            out[1], out[2] = linear_backward(dh, Act8(x8, of_x, ctx.fmt), types_[1], bias=needs[2])
         if needs[0]:
             out[0] = _input_grad(dh, w1, types_[0])
         for k in (2, 4):
