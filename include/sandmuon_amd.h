@@ -528,10 +528,11 @@ int smx_act8_decode(const uint8_t *codes, const uint8_t *scales, int fmt,
                     int64_t rows, int64_t cols, int64_t pitch, void *out,
                     int dtype, int64_t out_stride, void *stream);
 
-/* smx_act8_gelu: y = GELU(h), exact form, in h's type, with h kept in 8 bits
- * for smx_act8_gelu_backward and, unless y_codes and y_scales are null, y
- * kept as it is stored (rounded to its type) for smx_act8_wgrad of the Linear
- * that receives it.  smx_act8_gelu_backward: dh = dy * GELU'(kept h). */
+/* smx_act8_gelu: y = GELU(h), exact form, in h's type; unless h_codes and
+ * h_scales are null, h kept in 8 bits for smx_act8_gelu_backward, and unless
+ * y_codes and y_scales are null, y kept as it is stored (rounded to its type)
+ * for smx_act8_wgrad of the Linear that receives it.
+ * smx_act8_gelu_backward: dh = dy * GELU'(kept h). */
 int smx_act8_gelu(const void *h, int dtype, int64_t rows, int64_t cols,
                   int64_t row_stride, int fmt, void *y, int64_t y_stride,
                   uint8_t *h_codes, uint8_t *h_scales, uint8_t *y_codes,

@@ -102,11 +102,12 @@ def decode(saved: Act8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     return _native.torch_ops().act8_decode(saved.data, saved.shape, FORMATS[saved.fmt], dtype)
 
 
-def gelu_forward(h: torch.Tensor, fmt: str = "int8",
-                 keep_output: bool = True) -> Tuple[torch.Tensor, Act8, Optional[Act8]]:
-    """(GELU(h), h kept, the GELU's output kept or None) in one pass."""
-    y, kept_h, kept_y = _native.torch_ops().act8_gelu(h, _fmt(fmt, "act8.gelu_forward"), keep_output)
-    return y, Act8(kept_h, h.shape, fmt), Act8(kept_y, h.shape, fmt) if keep_output else None
+def gelu_forward(h: torch.Tensor, fmt: str = "int8", keep_output: bool = True,
+                 keep_input: bool = True) -> Tuple[torch.Tensor, Optional[Act8], Optional[Act8]]:
+    """(GELU(h), h kept, the GELU's output kept) in one pass, None for what is
+    not to be kept."""
+    y, *kept = _native.torch_ops().act8_gelu(h, _fmt(fmt, "act8.gelu_forward"), keep_input, keep_output)
+    return (y, *(None if data is None else Act8(data, h.shape, fmt) for data in kept))
 
 
 def gelu_backward(dy: torch.Tensor, saved: Act8) -> torch.Tensor:
@@ -191,22 +192,22 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
 class _Gelu(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, h, fmt):
-        y, kept, _ = gelu_forward(h, fmt, keep_output=False)
-        ctx.save_for_backward(kept.data)
-        ctx.kept = kept.shape, kept.fmt
+    def forward(ctx, h, fmt, grad):
+        y, kept, _ = gelu_forward(h, fmt, keep_output=False, keep_input=grad and ctx.needs_input_grad[0])
+        ctx.save_for_backward(_data(kept))
+        ctx.kept = h.shape, fmt
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        return gelu_backward(grad, Act8(*ctx.saved_tensors, *ctx.kept)), None
+        return gelu_backward(grad, Act8(*ctx.saved_tensors, *ctx.kept)), None, None
 
 
 def gelu(h: torch.Tensor, fmt: str = "int8") -> torch.Tensor:
     """F.gelu (exact form) whose input is kept in 8 bits."""
     _fmt(fmt, "act8.gelu")
-    return _Gelu.apply(h, fmt)
+    return _Gelu.apply(h, fmt, torch.is_grad_enabled())
 
 
 class _Mlp(torch.autograd.Function):
@@ -217,9 +218,8 @@ class _Mlp(torch.autograd.Function):
         x_lp, w1, b1, w2, b2 = (_cast(t, x.device.type) for t in (x, fc_w, fc_b, proj_w, proj_b))
         with torch.autocast(device_type=x.device.type, enabled=False):
             kept_x = encode(x_lp, fmt) if needs[1] or needs[2] else None
-            y, kept_h, kept_y = gelu_forward(F.linear(x_lp, w1, b1), fmt, keep_output=needs[3] or needs[4])
-            if not any(needs[:3]):
-                kept_h = None
+            y, kept_h, kept_y = gelu_forward(F.linear(x_lp, w1, b1), fmt, keep_output=needs[3] or needs[4],
+                                             keep_input=any(needs[:3]))
             out = F.linear(y, w2, b2)
         ctx.save_for_backward(w1 if needs[0] else None, w2 if any(needs[:3]) else None, *map(_data, (kept_x, kept_h, kept_y)))
         ctx.shapes, ctx.fmt = (x.shape, y.shape), fmt

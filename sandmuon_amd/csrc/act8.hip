@@ -182,7 +182,9 @@ __device__ __forceinline__ float gelu_slope(float h) {
   return fmaf(h, n.e * kPhi0, 0.5f + copysignf(0.5f - n.q, h));
 }
 
-enum Act8Op : int { kActEncode = 0, kActGelu = 1, kActDecode = 2, kActGeluBack = 3 };
+// (the GELU that keeps no input is a kernel of its own: a branch on the pointer cost
+// the other one 2%)
+enum Act8Op : int { kActEncode = 0, kActGelu = 1, kActDecode = 2, kActGeluBack = 3, kActGeluOut = 4 };
 
 template <int DT, int FMT, int OP>
 __global__ void __launch_bounds__(256) act8_kernel(Act8Args a) {
@@ -193,10 +195,10 @@ __global__ void __launch_bounds__(256) act8_kernel(Act8Args a) {
   const int64_t step = static_cast<int64_t>(gridDim.y) * blockDim.y;
   for (int64_t r = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; r < a.rows; r += step) {
     float v[8] = {};
-    if constexpr (OP == kActEncode || OP == kActGelu) {
+    if constexpr (OP == kActEncode || OP == kActGelu || OP == kActGeluOut) {
       if (n > 0) E::load(a.x, r * a.x_stride + 8 * chunk, n, v);
-      act8_put<FMT>(v, a.x8, r, a.pitch, chunk);
-      if constexpr (OP == kActGelu) {
+      if constexpr (OP != kActGeluOut) act8_put<FMT>(v, a.x8, r, a.pitch, chunk);
+      if constexpr (OP != kActEncode) {
         // (the output is kept as it is stored: rounded to its type first)
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = gelu_of<DT>(v[k]);
@@ -313,14 +315,15 @@ extern "C" int smx_act8_gelu(const void *h, int dtype, int64_t rows, int64_t col
   if (rows == 0 || cols == 0) return SMX_OK;
   ACT8_TRY(act8_check_tensor(what, h, rows, cols, row_stride));
   ACT8_TRY(act8_check_tensor(what, y, rows, cols, y_stride));
-  ACT8_TRY(act8_check_codes(what, h_codes, h_scales));
-  SMX_REQUIRE((y_codes == nullptr) == (y_scales == nullptr), SMX_EINVAL,
-              "act8_gelu: the output's codes and scales must both be given or both be null");
+  SMX_REQUIRE((h_codes == nullptr) == (h_scales == nullptr) && (y_codes == nullptr) == (y_scales == nullptr), SMX_EINVAL,
+              "act8_gelu: codes and scales must both be given or both be null");
+  if (h_codes) ACT8_TRY(act8_check_codes(what, h_codes, h_scales));
   if (y_codes) ACT8_TRY(act8_check_codes(what, y_codes, y_scales));
   Act8Args a{};
   a.x = h, a.y = y, a.x8 = {h_codes, h_scales}, a.y8 = {y_codes, y_scales};
   a.rows = rows, a.cols = cols, a.pitch = pitch, a.x_stride = row_stride, a.y_stride = y_stride;
-  return act8_launch<kActGelu>(a, dtype, fmt, static_cast<hipStream_t>(stream), what);
+  const auto st = static_cast<hipStream_t>(stream);
+  return h_codes ? act8_launch<kActGelu>(a, dtype, fmt, st, what) : act8_launch<kActGeluOut>(a, dtype, fmt, st, what);
 }
 
 extern "C" int smx_act8_gelu_backward(const void *dy, int dtype, int64_t rows, int64_t cols, int64_t dy_stride,

@@ -513,18 +513,19 @@ Tensor act8_decode(const Tensor &data, at::IntArrayRef shape, int64_t fmt, torch
   return out;
 }
 
-std::tuple<Tensor, Tensor, OptTensor> act8_gelu(const Tensor &h, int64_t fmt, bool keep_output) {
+std::tuple<Tensor, OptTensor, OptTensor> act8_gelu(const Tensor &h, int64_t fmt, bool keep_input, bool keep_output) {
   const Tensor r = rows2d(h, "act8.gelu_forward");
   const Tensor y = at::empty(h.sizes(), r.options());
-  const Kept kh = Kept::for_rows(r, r.size(0), r.size(1));
-  std::optional<Kept> ky;
-  if (keep_output) ky = Kept::for_rows(r, kh.rows, kh.cols);
+  const int64_t rows = r.size(0), cols = r.size(1), pitch = (cols + 31) / 32 * 32;
+  std::optional<Kept> kh, ky;
+  if (keep_input) kh = Kept::for_rows(r, rows, cols);
+  if (keep_output) ky = Kept::for_rows(r, rows, cols);
   const c10::DeviceGuard guard(r.device());
-  check(smx_act8_gelu(r.data_ptr(), dtype_of(r), kh.rows, kh.cols, r.stride(0), static_cast<int>(fmt), y.data_ptr(), kh.cols,
-                      kh.codes(), kh.scales(), ky ? ky->codes() : nullptr, ky ? ky->scales() : nullptr, kh.pitch,
-                      stream_of(r)),
+  check(smx_act8_gelu(r.data_ptr(), dtype_of(r), rows, cols, r.stride(0), static_cast<int>(fmt), y.data_ptr(), cols,
+                      kh ? kh->codes() : nullptr, kh ? kh->scales() : nullptr, ky ? ky->codes() : nullptr,
+                      ky ? ky->scales() : nullptr, pitch, stream_of(r)),
         "smx_act8_gelu");
-  return {y, kh.data, ky ? OptTensor(ky->data) : std::nullopt};
+  return {y, kh ? OptTensor(kh->data) : std::nullopt, ky ? OptTensor(ky->data) : std::nullopt};
 }
 
 Tensor act8_gelu_backward(const Tensor &dy, const Tensor &data, at::IntArrayRef shape, int64_t fmt) {

@@ -1,0 +1,38 @@
+"""8-bit activations where no gradient is wanted: nothing is kept."""
+import pytest
+import torch
+
+from sandmuon_amd import act8
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_nothing_is_kept_without_gradients(device, dtype):
+    rows, cols = 2048, 1024
+    codes = rows * cols * 33 // 32
+    h = torch.randn(rows, cols, device=device).to(dtype)
+    w = (torch.randn(cols, cols, device=device) / 32).to(dtype)
+    leaf = h.clone().requires_grad_()
+    want = act8.gelu(leaf).detach(), act8.mlp(leaf, w, None, w, None).detach()
+    del leaf
+    out = h.numel() * h.element_size()
+    torch.cuda.synchronize()
+
+    def peak(f):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        start = torch.cuda.memory_allocated()
+        y = f()
+        return y, torch.cuda.max_memory_allocated() - start
+
+    for ctx in (torch.no_grad(), torch.enable_grad()):  # (nothing here requires a gradient either)
+        with ctx:
+            y, more = peak(lambda: act8.gelu(h))
+            assert torch.equal(y, want[0]) and more < out + codes // 2
+            y, more = peak(lambda: act8.mlp(h, w, None, w, None))
+            assert torch.equal(y, want[1]) and more < 3 * out + codes // 2
+    with torch.no_grad():
+        leaf = h.requires_grad_()
+        y, more = peak(lambda: act8.gelu(leaf))
+        assert torch.equal(y, want[0]) and more < out + codes // 2
