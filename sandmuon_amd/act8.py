@@ -127,8 +127,11 @@ def linear_backward(delta: torch.Tensor, saved: Act8, dtype: Optional[torch.dtyp
 
 # ------------------------------------------------- differentiable functions ---
 def _cast(t: Optional[torch.Tensor], device_type: str) -> Optional[torch.Tensor]:
-    """t as autocast would hand it to a Linear."""
+    """t as autocast would hand it to a Linear (float64 and whole numbers as they
+    are).  Each call casts its own; autocast keeps a weight's cast for its region."""
     if t is None or not torch.is_autocast_enabled(device_type):
+        return t
+    if not t.is_floating_point() or t.dtype == torch.float64:
         return t
     return t.to(torch.get_autocast_dtype(device_type))
 

@@ -36,3 +36,16 @@ def test_nothing_is_kept_without_gradients(device, dtype):
         leaf = h.requires_grad_()
         y, more = peak(lambda: act8.gelu(leaf))
         assert torch.equal(y, want[0]) and more < out + codes // 2
+
+
+def test_float64_is_not_cast_by_autocast(device):
+    # as F.linear: autocast leaves float64 alone, and the types do not fit
+    w = torch.randn(8, 32, device=device, requires_grad=True)
+    x = torch.randn(4, 32, device=device, dtype=torch.float64)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        for f in (lambda: torch.nn.functional.linear(x, w), lambda: act8.linear(x, w),
+                  lambda: act8.mlp(x, w, None, w.t().contiguous(), None)):
+            with pytest.raises((RuntimeError, ValueError)):
+                f()
+
+
