@@ -148,6 +148,13 @@ def _data(saved: Optional[Act8]) -> Optional[torch.Tensor]:
     return None if saved is None else saved.data
 
 
+def _weight_grads(grad, saved: Act8, w_dtype, b_dtype, bias: bool):
+    """linear_backward with db in the bias's own type: where the two differ, both
+    come in FP32 and are rounded once."""
+    dw, db = linear_backward(grad, saved, w_dtype if not bias or b_dtype == w_dtype else torch.float32, bias=bias)
+    return dw.to(w_dtype), None if db is None else db.to(b_dtype)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, fmt, kept):
@@ -173,9 +180,7 @@ class _Linear(torch.autograd.Function):
         dx = _input_grad(grad, w, x_dtype) if needs[0] else None
         dw = db = None
         if needs[1] or needs[2]:
-            dw, db = linear_backward(grad, Act8(data, *ctx.kept), w_dtype, bias=needs[2])
-            if db is not None and b_dtype != w_dtype:
-                db = db.to(b_dtype)
+            dw, db = _weight_grads(grad, Act8(data, *ctx.kept), w_dtype, b_dtype, needs[2])
         return dx, dw if needs[1] else None, db, None, None
 
 
@@ -237,16 +242,13 @@ class _Mlp(torch.autograd.Function):
         of_x, of_h = ctx.shapes
         out = [None] * 7
         if needs[3] or needs[4]:
-            out[3], out[4] = linear_backward(grad, Act8(y8, of_h, ctx.fmt), types_[3], bias=needs[4])
+            out[3], out[4] = _weight_grads(grad, Act8(y8, of_h, ctx.fmt), types_[3], types_[4], needs[4])
         if any(needs[:3]):
             dh = gelu_backward(_input_grad(grad, w2, grad.dtype), Act8(h8, of_h, ctx.fmt))
         if needs[1] or needs[2]:
-            out[1], out[2] = linear_backward(dh, Act8(x8, of_x, ctx.fmt), types_[1], bias=needs[2])
+            out[1], out[2] = _weight_grads(dh, Act8(x8, of_x, ctx.fmt), types_[1], types_[2], needs[2])
         if needs[0]:
             out[0] = _input_grad(dh, w1, types_[0])
-        for k in (2, 4):
-            if out[k] is not None and out[k].dtype != types_[k]:
-                out[k] = out[k].to(types_[k])
         return tuple(g if k < 5 and needs[k] else None for k, g in enumerate(out))
 
 

@@ -49,3 +49,25 @@ def test_float64_is_not_cast_by_autocast(device):
                 f()
 
 
+
+
+def test_bias_gradient_is_rounded_once(device):
+    # a bias of more bits than its weight: db in its own type, not through the weight's
+    x = torch.randn(300, 64, device=device)
+    w = (torch.randn(40, 64, device=device) / 8).to(torch.bfloat16).requires_grad_()
+    b = torch.zeros(40, device=device, requires_grad=True)
+    proj = (torch.randn(24, 40, device=device) / 8).to(torch.bfloat16).requires_grad_()
+    c = torch.zeros(24, device=device, requires_grad=True)
+    cot = torch.randn(300, 24, device=device).to(torch.bfloat16)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = act8.mlp(x, w, b, proj, c)
+        z = act8.linear(x, w, b)
+    y.backward(cot)
+    want = cot.double().sum(0)
+    # an FP32 sum of 300 terms: 308 * 2^-24 of their magnitudes
+    assert ((c.grad.double() - want).abs() <= 308 * 2.0 ** -24 * cot.double().abs().sum(0)).all()
+    b.grad = None
+    cot = torch.randn(300, 40, device=device).to(torch.bfloat16)
+    z.backward(cot)
+    assert ((b.grad.double() - cot.double().sum(0)).abs() <= 308 * 2.0 ** -24 * cot.double().abs().sum(0)).all()
+    assert w.grad.dtype == torch.bfloat16 and b.grad.dtype == torch.float32
