@@ -27,7 +27,7 @@ FP32.  Double backward is not supported.
 """
 from __future__ import annotations
 
-import types
+import functools
 from typing import Callable, Optional, Tuple
 
 import torch
@@ -260,6 +260,12 @@ def mlp(x: torch.Tensor, fc_weight: torch.Tensor, fc_bias: Optional[torch.Tensor
     return _Mlp.apply(x, fc_weight, fc_bias, proj_weight, proj_bias, fmt, torch.is_grad_enabled())
 
 
+def _checkpointed_forward(module: nn.Linear, fmt: str, x: torch.Tensor, kept: Optional[Act8] = None) -> torch.Tensor:
+    if torch.is_grad_enabled() and x.is_cuda:
+        return linear(x, module.weight, module.bias, fmt, kept)
+    return F.linear(x, module.weight, module.bias)
+
+
 class CheckpointedLinears:
     """Handle of ``checkpoint_linears``; ``close()`` restores the forwards."""
 
@@ -280,16 +286,12 @@ def checkpoint_linears(model: nn.Module, module_filter: Optional[Callable[[str, 
     before; a module whose forward is replaced already is left as it is."""
     _fmt(fmt, "act8.checkpoint_linears")
 
-    def forward(module: nn.Linear, x: torch.Tensor, kept: Optional[Act8] = None) -> torch.Tensor:
-        if torch.is_grad_enabled() and x.is_cuda:
-            return linear(x, module.weight, module.bias, fmt, kept)
-        return F.linear(x, module.weight, module.bias)
-
     chosen = {}
     for name, module in model.named_modules():
         if type(module) is not nn.Linear or "forward" in module.__dict__:
             continue
         if module_filter is None or module_filter(name, module):
-            module.forward = types.MethodType(forward, module)
+            # (a partial of a module's function: pickled and copied models keep it)
+            module.forward = functools.partial(_checkpointed_forward, module, fmt)
             chosen[name] = module
     return CheckpointedLinears(chosen)

@@ -1,4 +1,5 @@
-"""8-bit activations where no gradient is wanted: nothing is kept."""
+"""8-bit activations around the training step: nothing kept where no gradient is
+wanted, types under autocast and of biases, copies of a model."""
 import pytest
 import torch
 
@@ -71,3 +72,26 @@ def test_bias_gradient_is_rounded_once(device):
     z.backward(cot)
     assert ((b.grad.double() - cot.double().sum(0)).abs() <= 308 * 2.0 ** -24 * cot.double().abs().sum(0)).all()
     assert w.grad.dtype == torch.bfloat16 and b.grad.dtype == torch.float32
+
+
+def test_checkpointed_models_pickle_and_copy(device):
+    import copy
+    import pickle
+    model = torch.nn.Sequential(torch.nn.Linear(64, 48), torch.nn.Linear(48, 8)).to(device)
+    act8.checkpoint_linears(model, fmt="e4m3")
+    x = torch.randn(32, 64, device=device)
+    want = model(x)
+    want.sum().backward()
+    for other in (pickle.loads(pickle.dumps(model)), copy.deepcopy(model)):
+        other.zero_grad(set_to_none=True)
+        assert "forward" in other[0].__dict__ and "forward" in other[1].__dict__
+        with torch.no_grad():  # (its own weights, not the first model's)
+            other[0].weight.add_(0)
+            other[1].bias.add_(1)
+        sizes = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: sizes.append(t.dtype) or t, lambda t: t):
+            y = other(x)
+        assert sizes.count(torch.uint8) == 2
+        assert torch.allclose(y, want + 1)
+        y.sum().backward()
+        assert torch.equal(other[0].weight.grad, model[0].weight.grad)
