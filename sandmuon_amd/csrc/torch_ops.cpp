@@ -86,6 +86,14 @@ void no_double_backward(const char *what) {
   TORCH_CHECK(!torch::GradMode::is_enabled(), what, ": its gradient cannot be differentiated (create_graph)");
 }
 
+// Nor has anything here a forward-mode one: a tangent is refused where no autograd
+// function sees it, and the result would count as a constant.
+void no_tangent(const char *what, std::initializer_list<const OptTensor *> inputs) {
+  for (const OptTensor *t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->has_value() || !(*t)->defined() || !(*t)->_fw_grad(0).defined(), what,
+                                ": no forward-mode derivative");
+}
+
 // ------------------------------------------------------ qk_norm_rotary ---
 struct QkRest {
   int64_t position0, style;
@@ -202,6 +210,8 @@ std::tuple<Tensor, Tensor> qk_norm_rotary(Tensor q, Tensor k, OptTensor qw, OptT
   kw = checked_weight(kw, k, "k_weight");
   const OptTensor others[] = {k, cos, sin};
   same_device(what, q, {&others[0], &others[1], &others[2], &qw, &kw, &positions});
+  const OptTensor first = q;
+  no_tangent(what, {&first, &others[0], &others[1], &others[2], &qw, &kw});
   if (positions.has_value()) {
     TORCH_CHECK_VALUE(integral(*positions) && (positions->dim() == 1 || positions->dim() == 2), what, ": positions ",
                       positions->sizes(), " ", positions->scalar_type(), "; expected integers [seq] or [batch, seq]");
@@ -248,8 +258,9 @@ void check_logits(const char *what, Tensor *logits, Tensor *targets, OptTensor *
                       ": mask ", (*mask)->sizes(), " ", type, "; expected bool [batch, seq]");
     *mask = (*mask)->contiguous();
   }
-  const OptTensor t = *targets;
+  const OptTensor t = *targets, z = *logits;
   same_device(what, *logits, {&t, mask});
+  no_tangent(what, {&z});
   *logits = apart_rows(*logits);
   *targets = targets->to(torch::kInt64).contiguous();
 }
