@@ -41,7 +41,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     integer tensor [seq] or [batch, seq]; a position outside the tables gives
     NaN.  Weights: [dim], or None for ones.  out: (q', k') to write into, of
     any strides with a unit last one (slots of a cache, or q and k
-    themselves), not under autograd.  Statistics and products are FP32, rounded
+    themselves, but no other overlap with what is read), not under autograd.  cos
+    and sin are constants: no gradient.  Statistics and products are FP32, rounded
     once to q's type."""
     code = STYLES.get(style)
     if code is None:

@@ -10,6 +10,7 @@
 // libsandmuon_amd.so, and errors are its status and message.
 #include <torch/extension.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 
@@ -236,10 +237,18 @@ std::tuple<Tensor, Tensor> qk_norm_rotary(Tensor q, Tensor k, OptTensor qw, OptT
         TORCH_CHECK_VALUE(o.size(d) <= 1 || o.stride(d) != 0 || o.numel() == 0, what, ": out of strides ", o.strides(),
                           " names places twice");
     }
+    // written while the other side, or another place of its own, is still read
+    const auto &[oq, ok] = *out;
+    at::assert_no_partial_overlap(oq, q);
+    at::assert_no_partial_overlap(ok, k);
+    at::assert_no_overlap(oq, k);
+    at::assert_no_overlap(ok, q);
+    at::assert_no_overlap(oq, ok);
   } else {
     out = {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options())};
   }
-  qk_forward(q, k, qw, kw, cos, sin, positions, {position0, style, eps}, std::get<0>(*out), std::get<1>(*out));
+  const auto &[oq, ok] = *out;
+  qk_forward(q, k, qw, kw, cos, sin, positions, {position0, style, eps}, oq, ok);
   return *out;
 }
 
