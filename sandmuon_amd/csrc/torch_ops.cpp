@@ -227,7 +227,8 @@ std::tuple<Tensor, Tensor> qk_norm_rotary(Tensor q, Tensor k, OptTensor qw, OptT
     const auto y = QkNormRotary::apply(q, k, qw, kw, cos, sin, positions, position0, eps, style);
     return {y[0], y[1]};
   }
-  if (out.has_value()) {
+  const bool given = out.has_value();
+  if (given) {
     for (const auto &[o, x] : {std::tie(std::get<0>(*out), q), std::tie(std::get<1>(*out), k)}) {
       TORCH_CHECK_VALUE(o.sizes() == x.sizes() && o.scalar_type() == x.scalar_type() && o.device() == x.device() &&
                             (o.size(3) <= 1 || o.stride(3) == 1),
@@ -236,6 +237,8 @@ std::tuple<Tensor, Tensor> qk_norm_rotary(Tensor q, Tensor k, OptTensor qw, OptT
       for (int d = 0; d < 3; ++d)
         TORCH_CHECK_VALUE(o.size(d) <= 1 || o.stride(d) != 0 || o.numel() == 0, what, ": out of strides ", o.strides(),
                           " names places twice");
+      TORCH_CHECK_VALUE(!torch::GradMode::is_enabled() || !o.requires_grad(), what,
+                        ": out= that requires a gradient is not supported under autograd");
     }
     // written while the other side, or another place of its own, is still read
     const auto &[oq, ok] = *out;
@@ -249,6 +252,8 @@ std::tuple<Tensor, Tensor> qk_norm_rotary(Tensor q, Tensor k, OptTensor qw, OptT
   }
   const auto &[oq, ok] = *out;
   qk_forward(q, k, qw, kw, cos, sin, positions, {position0, style, eps}, oq, ok);
+  // (a graph that saved what was there notices)
+  if (given) oq.unsafeGetTensorImpl()->bump_version(), ok.unsafeGetTensorImpl()->bump_version();
   return *out;
 }
 

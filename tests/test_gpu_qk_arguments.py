@@ -20,3 +20,31 @@ def test_out_over_other_operands_is_refused(device):
     a, b = fused[:, :, 0], fused[:, :, 1]
     got = qk_norm_rotary(a, b, None, None, cos, sin, out=(a, b))
     assert torch.equal(got[0], want[0]) and torch.equal(fused[:, :, 1], want[1])
+
+
+def test_out_raises_its_version(device):
+    cos, sin = rotary_tables(8, 16, device=device)
+    q, k = torch.randn(1, 4, 2, 16, device=device), torch.randn(1, 4, 2, 16, device=device)
+    scale = torch.ones(16, device=device, requires_grad=True)
+    y = q * scale  # saves q
+    versions = q._version, k._version
+    with torch.no_grad():
+        qk_norm_rotary(q, k, None, None, cos, sin, out=(q, k))
+    assert q._version > versions[0] and k._version > versions[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_out_that_requires_a_gradient(device):
+    cos, sin = rotary_tables(8, 16, device=device)
+    q, k = torch.randn(1, 4, 2, 16, device=device), torch.randn(1, 4, 2, 16, device=device)
+    out = torch.empty_like(q).requires_grad_(), torch.empty_like(k)
+    with pytest.raises(ValueError, match="out="):
+        qk_norm_rotary(q, k, None, None, cos, sin, out=out)
+    want = qk_norm_rotary(q, k, None, None, cos, sin)
+    with torch.no_grad():
+        assert torch.equal(qk_norm_rotary(q, k, None, None, cos, sin, out=out)[0], want[0])
+    with torch.inference_mode():
+        a, b = q.clone(), k.clone()
+        qk_norm_rotary(a, b, None, None, cos, sin, out=(a, b))
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1])
