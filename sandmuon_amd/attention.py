@@ -7,6 +7,7 @@ are one kernel launch each (two in the backward with weight gradients).
 """
 from __future__ import annotations
 
+import operator
 from typing import Optional, Tuple, Union
 
 import torch
@@ -49,5 +50,5 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
         raise ValueError(f"qk_norm_rotary: unknown style {style!r}; expected one of {sorted(STYLES)}")
     position0 = 0
     if positions is not None and not isinstance(positions, torch.Tensor):
-        positions, position0 = None, int(positions)
+        positions, position0 = None, operator.index(positions)
     return _native.torch_ops().qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, position0, eps, code, out)

@@ -48,3 +48,12 @@ def test_out_that_requires_a_gradient(device):
         a, b = q.clone(), k.clone()
         qk_norm_rotary(a, b, None, None, cos, sin, out=(a, b))
         assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+
+
+def test_first_position_is_a_whole_number(device):
+    cos, sin = rotary_tables(8, 16, device=device)
+    q = torch.randn(1, 2, 1, 16, device=device)
+    with pytest.raises(TypeError):
+        qk_norm_rotary(q, q, None, None, cos, sin, 2.5)
+    want = qk_norm_rotary(q, q, None, None, cos, sin, torch.tensor([3, 4], device=device))
+    assert torch.equal(qk_norm_rotary(q, q, None, None, cos, sin, 3)[0], want[0])
