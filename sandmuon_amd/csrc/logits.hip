@@ -528,9 +528,9 @@ __global__ void __launch_bounds__(1024) preference_kernel(PreferenceArgs a, int 
       if (a.smoothing < 1) loss += (1 - a.smoothing) * (soft - (m > 0.f ? 0.f : m));
       if (a.smoothing > 0) loss += a.smoothing * (soft + (m < 0.f ? 0.f : m));
       a.margins[p] = m;
-      // sigmoid(m) = 1 / (1 + e) or e / (1 + e)
-      const double up = static_cast<double>(m > 0.f ? 1.f : e) / (1.0 + e);
-      const double slope = a.beta * (up - (1 - a.smoothing)) / a.pairs;
+      // sigmoid(m) and sigmoid(-m) are 1 / (1 + e) and e / (1 + e) or the other way round
+      const double up = static_cast<double>(m > 0.f ? 1.f : e) / (1.0 + e), down = static_cast<double>(m > 0.f ? e : 1.f) / (1.0 + e);
+      const double slope = a.beta * (a.smoothing * up - (1 - a.smoothing) * down) / a.pairs;
       a.coef[p] = static_cast<float>(slope);
       a.coef[p + a.pairs] = static_cast<float>(-slope);
     }

@@ -12,7 +12,7 @@ the roundings' sum."""
 import pytest
 import torch
 
-from sandmuon_amd import losses
+from sandmuon_amd import _native, losses
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,22 @@ def test_margins_of_long_sequences(device, seed):
     one_sided = 2.0 ** -26 * (live[:pairs] - live[pairs:]).abs()
     bar = beta * (one_sided + 4 * (each[:pairs] + each[pairs:]).sqrt()) + 2.0 ** -23 * want.abs()
     assert ((margins.double() - want).abs() <= bar).all()
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 1.0, 0.25])
+def test_slopes_of_large_margins(device, smoothing):
+    # d loss / d lp is beta (s sigmoid(m) - (1 - s) sigmoid(-m)) / pairs, whatever is left of it:
+    # FP32 roundings of m (2^-24 of it), of exp(-|m|) and of the result
+    margins = torch.tensor([0.0, 0.3, -0.3, 9.0, -9.0, 20.0, -20.0, 33.0, 45.0, -45.0, 80.0, -80.0])
+    pairs, beta = len(margins), 0.5
+    lp = torch.cat([margins / beta, torch.zeros(pairs)])[:, None].contiguous().to(device)
+    loss, got = torch.empty((), device=device), torch.empty(pairs, device=device)
+    coef = torch.empty(2 * pairs, device=device)
+    rc = _native.lib().smx_preference_loss(lp.data_ptr(), torch.zeros_like(lp).data_ptr(), None, pairs, 1, beta, smoothing,
+                                           loss.data_ptr(), got.data_ptr(), coef.data_ptr(), _native.stream_of(lp.device))
+    assert rc == 0 and torch.equal(got.cpu(), margins)
+    m = margins.double()
+    want = beta * (smoothing * torch.sigmoid(m) - (1 - smoothing) * torch.sigmoid(-m)) / pairs
+    bar = (2.0 ** -22 + 2.0 ** -24 * m.abs()) * (smoothing * torch.sigmoid(m) + (1 - smoothing) * torch.sigmoid(-m)) * beta / pairs
+    for side, sign in ((coef[:pairs], 1), (coef[pairs:], -1)):
+        assert ((side.cpu().double() - sign * want).abs() <= bar + 1e-45).all()
