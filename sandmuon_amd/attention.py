@@ -23,6 +23,8 @@ def rotary_tables(positions: int, rot: int, base: float = 10000.0,
                   device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
     """cos and sin [positions, rot / 2] (float32) of the angles position *
     base^(-2p / rot)."""
+    if positions < 0 or rot < 0 or rot % 2:
+        raise ValueError(f"rotary_tables: {positions} positions of {rot} elements; expected an even number in pairs")
     freq = base ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
     angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
     return angle.cos().float(), angle.sin().float()
