@@ -16,12 +16,13 @@
 // write FP32 partial tiles that a second launch adds in order, so the result
 // does not depend on timing.
 //
-// Measured, BF16 cotangents, with db: 8192 x 2048 -> 8192 253 us in e4m3 (1.09
-// PFLOP/s) and 287 us in int8, whose codes take 2.5 vector instructions an element
-// to widen where e4m3 takes half of one; 16384 x 768 -> 3072 92 and 97 us; 16384 x
-// 768 -> 768 (small tiles, 14 splits) 38 us, 7 of them the join.  The wide tile is
-// bound by MFMA issue and the clock held under it (MFMAs busy 41% of the cycles,
-// LDS 31%), the small one by staging (28%).
+// Measured, BF16 cotangents, with db, calls back to back: 8192 x 2048 -> 8192 246 us
+// in e4m3 (1.12 PFLOP/s; 282-317 us among other kernels, at lower clocks) and 257 us
+// in int8, whose codes take 2.5 vector instructions an element to widen where e4m3
+// takes half of one; 16384 x 768 -> 3072 95 and 96 us; 16384 x 768 -> 768 (small
+// tiles, 14 splits) 41 us, 7 of them the join.  The wide tile is bound by MFMA issue
+// and the clock held under it (MFMAs busy 41% of the cycles, LDS 31%), the small one
+// by staging (28%).
 #include "act8.h"
 
 #include <algorithm>

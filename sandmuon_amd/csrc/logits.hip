@@ -6,11 +6,12 @@
 // kept apart: a row of values as large as their type's lowest has no room for
 // the sum's logarithm beside them.)
 // Bound by HBM: every row is read once and its gradient written once; a row's
-// exponentials are made twice, some 17 vector instructions an element, half of
+// exponentials are made twice, some 19 vector instructions an element, half of
 // the time.  Measured at 8 x 1024 x 50257 bf16, 30% of the tokens masked: the
-// policy loss with its gradient 283 us (1.40 GB, 4.9 TB/s), log probabilities
-// alone 100 us (5.7 TB/s), their gradient 257 us (5.4 TB/s, part of it read from
-// the last cache).
+// policy loss with its gradient 285 us (1.40 GB, 4.9 TB/s), log probabilities
+// alone 96-100 us (5.7-6 TB/s), their gradient 260 us (5.4 TB/s, part of it read
+// from the last cache).  FP16 logits, whose policy gradient is made in the backward:
+// 384 us for both.
 #include "common.h"
 
 #include <algorithm>
@@ -221,7 +222,10 @@ struct Row {
 };
 
 // A row of any length, read again for each use: first the maximum and sum,
-// then the gradient.
+// then the gradient.  For rows past 256 KB, which a block's registers do not hold;
+// an element a thread at a time, bound by one load in flight and the running
+// maximum's two exponentials an element: log probabilities of 4 x 512 x 151936 bf16
+// 260 us (1.7 TB/s), their gradient 409 us (2.6 TB/s).
 template <int DT>
 struct LongRow {
   static constexpr int NT = 1024;

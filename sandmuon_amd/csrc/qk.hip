@@ -240,7 +240,9 @@ __global__ void __launch_bounds__(kQkThreads) qk_kernel(QkArgs a) {
 
 // --------------------------------------------------------- any geometry ---
 // Dimensions, strides and addresses of any kind: a wave owns a vector and
-// goes over its elements three times, one (or one pair) a lane.
+// goes over its elements three times, one (or one pair) a lane.  16 x 1024 tokens of
+// 12 + 12 heads of 60, bf16: forward 125 us, backward with weights 251 us (0.8 and
+// 0.6 TB/s, bound by single-element accesses; heads of 64 take the kernel above).
 template <int DT, bool BACK>
 __global__ void __launch_bounds__(kQkThreads) qk_any_kernel(QkArgs a, int half) {
   const QkSide &s = a.side[blockIdx.y];

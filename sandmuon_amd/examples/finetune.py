@@ -61,7 +61,7 @@ class Block(nn.Module):
     def forward(self, x, tables):
         x = x + self.attn(self.ln_1(x), tables)
         h = self.mlp["c_fc"](self.ln_2(x))
-        return x + self.mlp["c_proj"](act8.gelu(h) if torch.is_grad_enabled() else F.gelu(h))
+        return x + self.mlp["c_proj"](act8.gelu(h))
 
 
 class Policy(nn.Module):

@@ -6,7 +6,8 @@ Logits are [batch, seq, vocab] (float32, bfloat16 or float16, any strides with
 a unit last one); every statistic is FP32 or wider.  A token whose mask is
 False is not looked at, whatever it holds: its log probability and gradient
 are 0.  A live token's target outside the vocabulary makes its log probability
-and gradient NaN.
+and gradient NaN.  The logits alone get gradients; advantages and recorded log
+probabilities are constants.
 """
 from __future__ import annotations
 
